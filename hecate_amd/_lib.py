@@ -59,6 +59,12 @@ SIGNATURES = {
     "hmoe_norm_route": (i32, [P, P, P, P, P, P, P, P, P, P, f32, f32, f32, f32, P, i32, i32, i32, i32, i32, i32, P]),
     "hmoe_decode_combine_norm": (i32, [P, P, i32, P, P, P, P, f32, f32, f32, i32, i32, P]),
     "hmoe_norm_router": (i32, [P, P, f32, i32, P, i32, P, P, P, P]),
+    "hmoe_i8_quantize": (i32, [P, i32, i64, i32, i32, P, i64, P, P]),
+    "hmoe_i8_matmul": (i32, [P, i64, P, i32, P, i64, P, i32, i32, P, P, i32, i64, P]),
+    "hmoe_i8_linear_work_bytes": (sz, [i32, i32, i32]),
+    "hmoe_i8_linear": (i32, [P, i32, i64, i32, P, i64, P, i32, i32, P, P, i32, i64, P, P]),
+    "hmoe_i8_mlp_work_bytes": (sz, [i32, i32, i32]),
+    "hmoe_i8_mlp": (i32, [P, i32, i64, i32, i32, i32, P, P, P, P, P, P, P, i32, i64, P, P]),
     "hmoe_cpu_start": (i32, [P, i32, i32]),
     "hmoe_cpu_add_layer": (i32, [i32, i32, i32, P, P]),
     "hmoe_cpu_stats": (i32, [P, P]),

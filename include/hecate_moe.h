@@ -248,6 +248,30 @@ int hmoe_shared_forward(const void* x, int T, const void* sh_gw, const void* sh_
 int hmoe_shared_rows(const void* x, int T, const void* sh_gw, const void* sh_uw, const void* sh_dw, void* work, float* out,
                      int xf, void* stream);
 
+/* ---- products in 8-bit integers with a scale for each token and each output channel, and the gated MLP made of them (the
+ * reference keeps its shared expert as int8 rows with fp32 row scales, runtime/tier/tier_split.py:252-263, and reads it
+ * in its decode op only, moe4.cu:846-895) ----
+ * A row of x [M][K] is held as s = max |x| / 127 and q = 127 x / max |x| rounded half to even (a row of zeros: s = 0,
+ * q = 0; a row with a NaN or an infinity: s = NaN, q = 0, so its products are NaN). Weights w int8 [N][K], row-major, one
+ * fp32 scale a row. y[m][n] = s[m] ws[n] sum_k q[m][k] w[n][k] (+ bias[n]): the sum exact in int32, the rest in fp32,
+ * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131072; q, w and
+ * the workspace are 16-byte aligned and their row strides multiples of 16; x and y need their type's alignment only. M = 0 is
+ * a no-op. y overlaps no input. ---- */
+/* x as q and s (the step that linear and mlp begin with, for a caller with several products of the same rows) */
+int hmoe_i8_quantize(const void* x, int x_dtype, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* s, void* stream);
+/* the product of rows that are in 8 bits already; bias fp32 [N] or NULL */
+int hmoe_i8_matmul(const int8_t* q, int64_t ldq, const float* s, int M, const int8_t* w, int64_t ldw, const float* ws, int N, int K,
+                   const float* bias, void* y, int y_dtype, int64_t ldy, void* stream);
+/* quantize, then matmul, through a workspace of hmoe_i8_linear_work_bytes(M, N, K) */
+size_t hmoe_i8_linear_work_bytes(int M, int N, int K);
+int hmoe_i8_linear(const void* x, int x_dtype, int64_t ldx, int M, const int8_t* w, int64_t ldw, const float* ws, int N, int K,
+                   const float* bias, void* y, int y_dtype, int64_t ldy, void* work, void* stream);
+/* y [M][H] = linear(h; wd, sd) of h = silu(linear(x; wg, sg)) linear(x; wu, su) in fp32, quantised row by row;
+ * wg, wu [I][H], wd [H][I] */
+size_t hmoe_i8_mlp_work_bytes(int M, int H, int I);
+int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H, int I, const int8_t* wg, const int8_t* wu, const int8_t* wd,
+                const float* sg, const float* su, const float* sd, void* y, int y_dtype, int64_t ldy, void* work, void* stream);
+
 /* ---- residual + RMSNorm: runtime/tier/cn.cu and runtime/core/nr4_kernel.cuh ----
  * Every RMSNorm here uses the reduction order of the reference's rms_norm_kernel, which its fused kernels reproduce
  * bit for bit (cn.cu:1-6,21-31,80-103; nr4_kernel.cuh:4-9): a row is H / 4 = 1536 float4 columns, chain t of 1024
