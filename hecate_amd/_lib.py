@@ -65,6 +65,9 @@ SIGNATURES = {
     "hmoe_i8_linear": (i32, [P, i32, i64, i32, P, i64, P, i32, i32, P, P, i32, i64, P, P]),
     "hmoe_i8_mlp_work_bytes": (sz, [i32, i32, i32]),
     "hmoe_i8_mlp": (i32, [P, i32, i64, i32, i32, i32, P, P, P, P, P, P, P, i32, i64, P, P]),
+    "hmoe_moe8_work_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "hmoe_moe8_layer": (i32, [P, i32, i64, i32, P, P, i32, i32, ctypes.c_double, P, P, P, P, P, P, i32, i32, i32, i32, P, P, P, P, P, i32,
+                              i64, P, P]),
     "hmoe_cpu_start": (i32, [P, i32, i32]),
     "hmoe_cpu_add_layer": (i32, [i32, i32, i32, P, P]),
     "hmoe_cpu_stats": (i32, [P, P]),

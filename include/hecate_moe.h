@@ -272,6 +272,20 @@ size_t hmoe_i8_mlp_work_bytes(int M, int H, int I);
 int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H, int I, const int8_t* wg, const int8_t* wu, const int8_t* wd,
                 const float* sg, const float* su, const float* sd, void* y, int y_dtype, int64_t ldy, void* work, void* stream);
 
+/* ---- a whole mixture-of-experts layer for up to 16 tokens, its experts in 8 bits (the formats and roundings above) ----
+ * Scores a = sigmoid(wr x) with the sums in 64 bits (wr fp32 [E][H]); sel the topk largest a + bias (bias fp32 [E] or NULL),
+ * equal ones in the order of their ids, a NaN last; rw = scale a / (sum of the selected a + 1e-20), fp32 (the selection of
+ * runtime/core/exl3_router.py:94-127). y [T][H] = the sum over the selected experts with lo <= id < lo + n of rw times
+ * their gated MLP (wg, wu [n][I][H], wd [n][H][I], scales [n][I], [n][I], [n][H]) and the shared expert's (sh_w / sh_s, host
+ * arrays of three device addresses, gate, up, down; both NULL without one). T <= 16, topk <= 16, E <= 512, H and I multiples
+ * of 16 up to 8192. wr and the weights are 16-byte aligned, the workspace (hmoe_moe8_work_bytes, 0 for sizes that are refused)
+ * 128-byte; a workspace made for more tokens serves fewer. T = 0 is a no-op. y overlaps no input. ---- */
+size_t hmoe_moe8_work_bytes(int T, int H, int I, int E, int topk);
+int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, const float* wr, const float* bias, int E, int topk, double scale,
+                    const int8_t* wg, const int8_t* wu, const int8_t* wd, const float* sg, const float* su, const float* sd, int n,
+                    int lo, int H, int I, const int8_t* const* sh_w, const float* const* sh_s, int64_t* sel, float* rw, void* y,
+                    int y_dtype, int64_t ldy, void* work, void* stream);
+
 /* ---- residual + RMSNorm: runtime/tier/cn.cu and runtime/core/nr4_kernel.cuh ----
  * Every RMSNorm here uses the reduction order of the reference's rms_norm_kernel, which its fused kernels reproduce
  * bit for bit (cn.cu:1-6,21-31,80-103; nr4_kernel.cuh:4-9): a row is H / 4 = 1536 float4 columns, chain t of 1024

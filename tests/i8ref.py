@@ -33,8 +33,8 @@ def product_bound(p, y, dtype):
 
 
 def mlp(q, a, wg, wu, wd, sg, su, sd):
-    """(y, slack): the gated MLP in 64 bits, and how far y may move because a gated value that lies within its own error of a
-    border between two whole numbers may be rounded to the other one.
+    """(y, slack, size): the gated MLP in 64 bits, how far y may move because a gated value that lies within its own error of a
+    border between two whole numbers may be rounded to the other one, and the sum of its terms' magnitudes.
 
     The error of h = silu(g) u, relative: g and u carry 4 u each; silu'(g) g / silu(g) = 1 + g (1 - sigmoid(g)) is at most
     1 + |g| in size; e^-g by exp2 of a rounded product carries (|g| + 2) u, counted twice for the hardware's exp2; the sum,
@@ -55,4 +55,4 @@ def mlp(q, a, wg, wu, wd, sg, su, sd):
     # row's largest value: at most |moved - y| (1 + err) + err |y| from y (4.01 u < err / 2; the roundings of y's own product
     # are product_bound's)
     slack = (near.astype(np.float64) @ np.abs(wn).T) * (top / 127.0) * np.abs(sdn) * (1 + err) + err * np.abs(y)
-    return y, slack
+    return y, slack, (np.abs(p) @ np.abs(wn).T) * (top / 127.0) * np.abs(sdn)

@@ -192,7 +192,7 @@ def test_mlp(dev, M, H, I, dtype, odt):
     for _ in range(2):                                    # (the second call finds the first's workspace)
         i8.mlp(x, wg, wu, wd, sg, su, sd, out, work)
     torch.cuda.synchronize()
-    y, slack = R.mlp(*R.rows8(x), wg, wu, wd, sg, su, sd)
+    y, slack, _ = R.mlp(*R.rows8(x), wg, wu, wd, sg, su, sd)
     d = np.abs(out.float().cpu().numpy() - y)
     b = R.product_bound(y, y, odt) + slack * (1 + 2 * R.HALF[odt])
     assert (d <= b).all(), (d.max(), np.argmax(d - b))
