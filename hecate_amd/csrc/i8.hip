@@ -1,7 +1,7 @@
 // i8.hip - products in 8-bit integers with a scale for each token and each output channel, and the gated MLP made of them
 // (hmoe_i8_quantize, hmoe_i8_matmul, hmoe_i8_linear, hmoe_i8_mlp):
 //   y[m][n] = s_x[m] s_w[n] sum_k q[m][k] w[n][k] (+ bias[n]), the sum exact in int32, the rest fp32, rounded once to y's type.
-#include "i8_dev.h"
+#include "i8_gemm.h"
 
 namespace hmoe {
 
@@ -36,89 +36,8 @@ __global__ void __launch_bounds__(256) i8_quant_kernel(const void* __restrict__ 
     }
 }
 
-// ---- products of any number of rows --------------------------------------------------------------------------------
-// Workgroup: 16 output channels (of one matrix, or of gate and up) x 16 MT tokens; its 8 waves split the depth, each with
-// its fragments straight from memory, and join their sums in LDS.
-struct I8Out
-{
-    void* y; int64_t ldy; int dt;
-    const float* xs; const float* ws; const float* ws2; const float* bias;
-};
-
-template <int MT, bool DUAL>
-__global__ void __launch_bounds__(512) i8_rows_kernel(const int8_t* __restrict__ q, int64_t ldq, const int8_t* __restrict__ w,
-                                                      const int8_t* __restrict__ w2, int64_t ldw, int M, int N, int K, I8Out o)
-{
-    constexpr int NM = DUAL ? 2 : 1;
-    __shared__ i32x4 red[8][NM * MT][64];
-    const int t = threadIdx.x, l = t & 63, wv = t >> 6;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-    const int n = min(n0 + (l & 15), N - 1);
-    const int8_t* wr[NM];
-    wr[0] = w + (size_t) n * ldw;
-    if (DUAL) wr[NM - 1] = w2 + (size_t) n * ldw;
-    const int8_t* qr[MT];
-    #pragma unroll
-    for (int j = 0; j < MT; ++j) qr[j] = q + (size_t) min(m0 + 16 * j + (l & 15), M - 1) * ldq;
-    i32x4 acc[NM][MT];
-    #pragma unroll
-    for (int a = 0; a < NM; ++a)
-        #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[a][j] = (i32x4) {0, 0, 0, 0};
-    // whole 128-byte lines to a wave
-    const int per = 2 * cdiv(cdiv(K, 128), 8);
-    const int c1 = min((wv + 1) * per, cdiv(K, 64));
-    #pragma unroll 2
-    for (int c = wv * per; c < c1; ++c)
-    {
-        const int k = 64 * c + 16 * (l >> 4);
-        const int ko = min(k, K - 16);
-        u32x4 av[NM];
-        #pragma unroll
-        for (int a = 0; a < NM; ++a)
-        {
-            av[a] = ld16(wr[a] + ko);
-            if (k != ko) av[a] = (u32x4) {0u, 0u, 0u, 0u};         // behind the depth: nothing
-        }
-        #pragma unroll
-        for (int j = 0; j < MT; ++j)
-        {
-            const u32x4 b = ld16(qr[j] + ko);
-            #pragma unroll
-            for (int a = 0; a < NM; ++a) acc[a][j] = mfma_i8(av[a], b, acc[a][j]);
-        }
-    }
-    #pragma unroll
-    for (int a = 0; a < NM; ++a)
-        #pragma unroll
-        for (int j = 0; j < MT; ++j) red[wv][a * MT + j][l] = acc[a][j];
-    __syncthreads();
-    for (int i = t; i < MT * 64; i += 512)
-    {
-        const int j = i >> 6, ll = i & 63, m = m0 + 16 * j + (ll & 15), nb = n0 + 4 * (ll >> 4);
-        i32x4 s[NM];
-        #pragma unroll
-        for (int a = 0; a < NM; ++a)
-        {
-            s[a] = red[0][a * MT + j][ll];
-            #pragma unroll
-            for (int v = 1; v < 8; ++v) s[a] += red[v][a * MT + j][ll];
-        }
-        if (m >= M) continue;
-        const float xs = o.xs[m];
-        #pragma unroll
-        for (int e = 0; e < 4; ++e)
-        {
-            if (nb + e >= N) continue;
-            float v = (float) s[0][e] * xs * o.ws[nb + e];
-            if (DUAL) v = swiglu(v, (float) s[NM - 1][e] * xs * o.ws2[nb + e]);
-            if (o.bias) v += o.bias[nb + e];
-            store_out(o.y, (size_t) m * o.ldy + nb + e, v, o.dt);
-        }
-    }
-}
-
-constexpr int I8_MAXK = 131072;              // 128 x 128 x K stays below 2^31
+constexpr int I8_MAXK = 131056;              // 128 x 128 x K stays below 2^31
+constexpr int64_t I8_MAXLD = 1 << 28;        // the product's kernel steps over 8 rows in 32 bits
 
 static int launch_quant(const void* x, int dt, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* s, hipStream_t st)
 {
@@ -132,14 +51,10 @@ static int launch_quant(const void* x, int dt, int64_t ldx, int M, int K, int8_t
     return HMOE_LAUNCHED("i8 quantize");
 }
 
-// one product, or (w2) gate and up with y = silu(gate) up in fp32
-static int launch_product(const int8_t* q, int64_t ldq, const int8_t* w, const int8_t* w2, int64_t ldw, int M, int N, int K,
-                          const I8Out& o, hipStream_t st)
+static I8Out out_of(void* y, int64_t ldy, int dt, const float* xs, const float* ws, const float* ws2, const float* bias)
 {
-    const dim3 g(cdiv(N, 16), cdiv(M, 64));
-    if (w2) i8_rows_kernel<4, true><<<g, 512, 0, st>>>(q, ldq, w, w2, ldw, M, N, K, o);
-    else i8_rows_kernel<4, false><<<g, 512, 0, st>>>(q, ldq, w, nullptr, ldw, M, N, K, o);
-    return HMOE_LAUNCHED("i8 product");
+    const bool vec = ((uintptr_t) y & 15) == 0 && (ldy * (dt == HMOE_DT_F32 ? 4 : 2)) % 16 == 0;
+    return {y, ldy, dt, xs, ws, ws2, bias, vec};
 }
 
 static bool is_dt(int dt) { return dt == HMOE_DT_F32 || dt == HMOE_DT_BF16 || dt == HMOE_DT_F16; }
@@ -159,7 +74,7 @@ static int check_x(const char* what, const void* x, int dt, int64_t ldx, int M, 
 static int check_w(const char* what, const int8_t* w, const float* ws, int64_t ldw, int N, int K)
 {
     HMOE_REQUIRE(N >= 1 && N <= (1 << 20), "%s: %d output channels: 1 to %d", what, N, 1 << 20);
-    HMOE_REQUIRE(w && ws && ((uintptr_t) w & 15) == 0 && ((uintptr_t) ws & 3) == 0 && ldw % 16 == 0 && rows_ok(N, ldw, K),
+    HMOE_REQUIRE(w && ws && ((uintptr_t) w & 15) == 0 && ((uintptr_t) ws & 3) == 0 && ldw % 16 == 0 && ldw < I8_MAXLD && rows_ok(N, ldw, K),
                  "%s: weights: null, not 16-byte aligned, or row stride %lld for depth %d", what, (long long) ldw, K);
     return HMOE_OK;
 }
@@ -202,13 +117,13 @@ extern "C" int hmoe_i8_matmul(const int8_t* q, int64_t ldq, const float* s, int 
     if (M == 0) return HMOE_OK;
     HMOE_REQUIRE(K >= 16 && K % 16 == 0 && K <= I8_MAXK, "i8_matmul: depth %d: a multiple of 16 up to %d", K, I8_MAXK);
     HMOE_REQUIRE(M > 0 && M <= (1 << 20), "i8_matmul: %d rows: up to %d", M, 1 << 20);
-    HMOE_REQUIRE(q && s && ((uintptr_t) q & 15) == 0 && ((uintptr_t) s & 3) == 0 && ldq % 16 == 0 && rows_ok(M, ldq, K),
+    HMOE_REQUIRE(q && s && ((uintptr_t) q & 15) == 0 && ((uintptr_t) s & 3) == 0 && ldq % 16 == 0 && ldq < I8_MAXLD && rows_ok(M, ldq, K),
                  "i8_matmul: q: null, not 16-byte aligned, or row stride %lld", (long long) ldq);
     if (int rc = check_w("i8_matmul", w, ws, ldw, N, K)) return rc;
     HMOE_REQUIRE(((uintptr_t) bias & 3) == 0, "i8_matmul: bias alignment");
     if (int rc = check_y("i8_matmul", y, y_dtype, ldy, M, N)) return rc;
     HMOE_REQUIRE(!overlap(q, M, ldq, K, 1, y, M, ldy, N, dt_size(y_dtype)), "i8_matmul: the output overlaps q");
-    return launch_product(q, ldq, w, nullptr, ldw, M, N, K, {y, ldy, y_dtype, s, ws, nullptr, bias}, (hipStream_t) stream);
+    return i8_product(q, ldq, w, ldw, M, N, K, out_of(y, ldy, y_dtype, s, ws, nullptr, bias), (hipStream_t) stream);
 }
 
 extern "C" size_t hmoe_i8_linear_work_bytes(int M, int N, int K)
@@ -232,7 +147,7 @@ extern "C" int hmoe_i8_linear(const void* x, int x_dtype, int64_t ldx, int M, co
     int8_t* q = (int8_t*) work;
     float* s = (float*) (q + up128((size_t) M * K));
     if (int rc = launch_quant(x, x_dtype, ldx, M, K, q, K, s, st)) return rc;
-    return launch_product(q, K, w, nullptr, ldw, M, N, K, {y, ldy, y_dtype, s, ws, nullptr, bias}, st);
+    return i8_product(q, K, w, ldw, M, N, K, out_of(y, ldy, y_dtype, s, ws, nullptr, bias), st);
 }
 
 // workspace: x in 8 bits and its scales, the gated rows in fp32, then in 8 bits with their scales
@@ -262,7 +177,7 @@ extern "C" int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H
     int8_t* qa = (int8_t*) act + up128((size_t) M * Id * 4);
     float* sa = (float*) (qa + up128((size_t) M * Id));
     if (int rc = launch_quant(x, x_dtype, ldx, M, Hd, q, Hd, s, st)) return rc;
-    if (int rc = launch_product(q, Hd, wg, wu, Hd, M, Id, Hd, {act, Id, HMOE_DT_F32, s, sg, su, nullptr}, st)) return rc;
+    if (int rc = i8_gated(q, Hd, wg, wu, Hd, M, Id, Hd, out_of(act, Id, HMOE_DT_F32, s, sg, su, nullptr), st)) return rc;
     if (int rc = launch_quant(act, HMOE_DT_F32, Id, M, Id, qa, Id, sa, st)) return rc;
-    return launch_product(qa, Id, wd, nullptr, Id, M, Hd, Id, {y, ldy, y_dtype, sa, sd, nullptr, nullptr}, st);
+    return i8_product(qa, Id, wd, Id, M, Hd, Id, out_of(y, ldy, y_dtype, sa, sd, nullptr, nullptr), st);
 }

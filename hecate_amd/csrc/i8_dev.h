@@ -144,9 +144,10 @@ __device__ __forceinline__ int dot16(u32x4 a, u32x4 b, int c)
 // gives NaN (inf 0), as g sigmoid(g) does.
 __device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
+// fp32 to a 16-bit type, to the nearest, ties to even (the hardware's conversions)
 __device__ __forceinline__ uint16_t to16(float v, int dt)
 {
-    return dt == HMOE_DT_BF16 ? hmoe_f2bf(v) : __builtin_bit_cast(uint16_t, (_Float16) v);
+    return dt == HMOE_DT_BF16 ? __builtin_bit_cast(uint16_t, (__bf16) v) : __builtin_bit_cast(uint16_t, (_Float16) v);
 }
 __device__ __forceinline__ void store_out(void* out, size_t i, float v, int dt)
 {

@@ -254,8 +254,8 @@ int hmoe_shared_rows(const void* x, int T, const void* sh_gw, const void* sh_uw,
  * A row of x [M][K] is held as s = max |x| / 127 and q = 127 x / max |x| rounded half to even (a row of zeros: s = 0,
  * q = 0; a row with a NaN or an infinity: s = NaN, q = 0, so its products are NaN). Weights w int8 [N][K], row-major, one
  * fp32 scale a row. y[m][n] = s[m] ws[n] sum_k q[m][k] w[n][k] (+ bias[n]): the sum exact in int32, the rest in fp32,
- * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131072; q, w and
- * the workspace are 16-byte aligned and their row strides multiples of 16; x and y need their type's alignment only. M = 0 is
+ * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131056; q, w and
+ * the workspace are 16-byte aligned and their row strides multiples of 16 (below 2^28 in a product); x and y need their type's alignment only. M = 0 is
  * a no-op. y overlaps no input. ---- */
 /* x as q and s (the step that linear and mlp begin with, for a caller with several products of the same rows) */
 int hmoe_i8_quantize(const void* x, int x_dtype, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* s, void* stream);

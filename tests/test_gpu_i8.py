@@ -147,15 +147,39 @@ def test_linear(dev, M, N, K, dtype, odt, pad):
 
 
 def test_extreme_weights_fill_the_accumulator(dev):
-    """-128 x -127 over a depth of 131072: the sum just fits 32 bits"""
-    K = 131072
+    """-128 x -128 over the largest depth: the sum just fits 32 bits"""
+    K = 131056
     for M in (1, 3, 33, 200):
-        q = torch.full((M, K), -127, dtype=torch.int8, device=dev)
+        q = torch.full((M, K), -128, dtype=torch.int8, device=dev)
         w = torch.full((20, K), -128, dtype=torch.int8, device=dev)
         one = torch.ones(M, device=dev)
         out = torch.empty((M, 20), device=dev)
         i8.matmul(q, one, w, torch.ones(20, device=dev), out)
-        assert bool((out == float(np.float32(127.0 * 128.0 * K))).all())
+        assert bool((out == float(np.float32(128.0 * 128.0 * K))).all())
+
+
+# sizes that fall on each of the product's tile shapes in turn (i8_gemm1.hip), whole tiles and ragged ones, the depth ending
+# inside a stage
+TILES = [(7, 4100, 80), (16, 4096, 1024), (17, 2050, 80), (30, 2048, 400), (33, 4100, 144), (64, 2080, 656), (100, 4100, 80), (65, 4096, 384),
+         (129, 6150, 80), (200, 4096, 144), (500, 4100, 80), (512, 4096, 128), (1000, 4100, 80), (1024, 4096, 144), (2000, 4100, 80),
+         (2048, 6144, 128), (4100, 2050, 336)]
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_matmul_tile_shapes(dev, M, N, K):
+    log("tiles", M, N, K)
+    g = torch.Generator().manual_seed(M + N + K)
+    q = torch.randint(-127, 128, (M, K), generator=g, dtype=torch.int8)
+    s = 0.01 + torch.rand(M, generator=g)
+    w, ws = weight(N, K, M + N)
+    bias = torch.randn(N, generator=g)
+    p = R.product(q.double().numpy(), s.double().numpy()[:, None] * 127.0, w, ws)
+    for odt, b in ((BF, bias), (F32, None), (F16, bias)):
+        buf = torch.full((M + 1, N + 8), 7.0, dtype=odt, device=dev)
+        i8.matmul(q.to(dev), s.to(dev), w, ws, buf[:M, :N], None if b is None else b.to(dev))
+        torch.cuda.synchronize()
+        check_out(buf[:M, :N], p, p if b is None else p + b.double().numpy())
+        assert bool((buf[M] == 7.0).all()) and bool((buf[:, N:] == 7.0).all())
 
 
 def test_rows_that_are_not_finite_stay_apart(dev):
@@ -178,7 +202,10 @@ def test_rows_that_are_not_finite_stay_apart(dev):
 
 
 MLPS = [(1, 6144, 2048), (1, 16, 16), (2, 144, 48), (4, 2048, 1408), (13, 512, 272), (16, 1024, 704), (40, 256, 144), (77, 2048, 512),
-        (150, 384, 1040), (300, 1024, 256), (16, 6144, 2048)]
+        (150, 384, 1040), (300, 1024, 256), (16, 6144, 2048),
+        # each of the gated product's tile shapes (i8_gemm2.hip)
+        (17, 80, 2064), (100, 1040, 1040), (40, 80, 4112), (65, 144, 4096), (129, 80, 6160), (200, 128, 2048), (300, 80, 6160), (512, 128, 4096),
+        (1000, 80, 4112), (2048, 144, 2048), (120, 6144, 2048)]
 
 
 @pytest.mark.parametrize("M,H,I", MLPS)

@@ -20,7 +20,7 @@ def test_quantize_refuses():
     refused(bad(dt=5), "dtype")
     refused(bad(K=24), "depth")
     refused(bad(K=0), "depth")
-    refused(bad(K=131088, ldx=131088, ldq=131088), "depth")
+    refused(bad(K=131072, ldx=131072, ldq=131072), "depth")
     refused(bad(M=-1), "rows")
     refused(bad(M=(1 << 20) + 1), "rows")
     refused(bad(x=None), "x address")
@@ -45,6 +45,8 @@ def test_matmul_refuses():
     refused(bad(N=0), "output channels")
     refused(bad(q=A + 4), "q:")
     refused(bad(ldq=65), "q:")
+    refused(bad(ldq=1 << 28), "q:")
+    refused(bad(ldw=1 << 28), "weights")
     refused(bad(w=None), "weights")
     refused(bad(w=3 * A + 8), "weights")
     refused(bad(ldw=48), "weights")
