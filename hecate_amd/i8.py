@@ -10,24 +10,37 @@ contiguous.
 Work runs on the current torch stream of x's device and allocates nothing; a workspace (linear_work, mlp_work) is the
 caller's, any contents work, and calls that share one must not overlap. Errors raise RuntimeError.
 """
+from functools import lru_cache
+
 import torch
 
-from ._lib import call, dt_of, lib, on_device, ptr, stream_of
+from ._lib import check, lib, on_device
+
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the dtype codes of include/hecate_moe.h (HMOE_DT_*)
+
+
+def _dt(what, t):
+    d = _DT.get(t.dtype)
+    if d is None:
+        raise RuntimeError(f"{what}: dtype {t.dtype} not supported here (float32, bfloat16, float16)")
+    return d
 
 
 def _rows(what, t, M, K, dtype=None):
     """the row stride of a [M, K] tensor whose rows are contiguous"""
-    if t.dim() != 2 or t.shape[0] != M or t.shape[1] != K or (K > 1 and t.stride(1) != 1) or (dtype is not None and t.dtype != dtype):
+    if t.shape != (M, K) or (K > 1 and t.stride(1) != 1) or (dtype is not None and t.dtype != dtype):
         raise RuntimeError(f"{what} must be [{M}, {K}]{'' if dtype is None else ' ' + str(dtype)} with contiguous rows, "
                            f"got {tuple(t.shape)} {t.dtype}")
+    if M <= 1:
+        return K
     ld = t.stride(0)
-    if M > 1 and ld < K:
+    if ld < K:
         raise RuntimeError(f"{what}: rows overlap (stride {ld})")
-    return max(ld, K)
+    return ld
 
 
 def _vec(what, t, n):
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{what} must be {n} contiguous fp32 values")
 
 
@@ -37,75 +50,92 @@ def _mat(what, w, N, K):
 
 
 def _work(what, t, nbytes):
-    if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < nbytes:
+    if t is None or t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < nbytes:
         raise RuntimeError(f"{what}: the workspace must be contiguous uint8 of at least {nbytes} bytes")
 
 
+def _two(what, x):
+    if x.dim() != 2:
+        raise RuntimeError(f"{what} must have two dimensions, got {tuple(x.shape)}")
+    return x.shape
+
+
+@lru_cache(maxsize=256)
+def _bytes(name, *sizes):
+    return int(getattr(lib(), name)(*sizes))
+
+
 def _run(dev, name, *args):
-    """the C entry on dev's current stream, with dev as the current device"""
-    if dev.index != torch.cuda.current_device():
+    """the C entry on dev's current stream, with dev as the current device (raw queries: a call of a few microseconds pays
+    for every Python object that it makes)"""
+    i = dev.index
+    if i != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            return call(name, *args, stream_of(dev))
-    call(name, *args, stream_of(dev))
+            rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        check(rc, name)
 
 
 def quantize(x, q, s):
     """x [M, K] (bf16, fp16 or fp32) as int8 q [M, K] and fp32 scales s [M]"""
     on_device("i8.quantize", x, q, s)
-    M, K = x.shape
+    M, K = _two("i8: x", x)
     ldx, ldq = _rows("i8.quantize: x", x, M, K), _rows("i8.quantize: q", q, M, K, torch.int8)
     _vec("i8.quantize: s", s, M)
-    _run(x.device, "hmoe_i8_quantize", ptr(x), dt_of(x), ldx, M, K, ptr(q), ldq, ptr(s))
+    _run(x.device, "hmoe_i8_quantize", x.data_ptr(), _dt("i8: x", x), ldx, M, K, q.data_ptr(), ldq, s.data_ptr())
     return q, s
 
 
 def matmul(q, s, w, ws, out, bias=None):
     """out [M, N] = s[m] ws[n] (q [M, K] w [N, K]^T) (+ bias [N] fp32) of rows that are in 8 bits already"""
     on_device("i8.matmul", q, s, w, ws, out, bias)
-    M, K = q.shape
-    N = w.shape[0]
+    M, K = _two("i8: q", q)
+    N = _two("i8: w", w)[0]
     ldq, ldy = _rows("i8.matmul: q", q, M, K, torch.int8), _rows("i8.matmul: out", out, M, N)
     _mat("i8.matmul: w", w, N, K)
     _vec("i8.matmul: s", s, M)
     _vec("i8.matmul: ws", ws, N)
     if bias is not None:
         _vec("i8.matmul: bias", bias, N)
-    _run(q.device, "hmoe_i8_matmul", ptr(q), ldq, ptr(s), M, ptr(w), K, ptr(ws), N, K, ptr(bias), ptr(out), dt_of(out), ldy)
+    _run(q.device, "hmoe_i8_matmul", q.data_ptr(), ldq, s.data_ptr(), M, w.data_ptr(), K, ws.data_ptr(), N, K,
+         None if bias is None else bias.data_ptr(), out.data_ptr(), _dt("i8: out", out), ldy)
     return out
 
 
 def linear_work(device, M, N, K):
     """workspace of linear for up to M rows"""
-    return torch.empty(max(int(lib().hmoe_i8_linear_work_bytes(M, N, K)), 16), dtype=torch.uint8, device=torch.device(device))
+    return torch.empty(max(_bytes("hmoe_i8_linear_work_bytes", M, N, K), 16), dtype=torch.uint8, device=torch.device(device))
 
 
 def linear(x, w, ws, out, work, bias=None):
     """out [M, N] = quantize(x [M, K]) w [N, K]^T (+ bias [N] fp32)"""
     on_device("i8.linear", x, w, ws, out, work, bias)
-    M, K = x.shape
-    N = w.shape[0]
+    M, K = _two("i8: x", x)
+    N = _two("i8: w", w)[0]
     ldx, ldy = _rows("i8.linear: x", x, M, K), _rows("i8.linear: out", out, M, N)
     _mat("i8.linear: w", w, N, K)
     _vec("i8.linear: ws", ws, N)
     if bias is not None:
         _vec("i8.linear: bias", bias, N)
-    _work("i8.linear", work, lib().hmoe_i8_linear_work_bytes(M, N, K))
-    _run(x.device, "hmoe_i8_linear", ptr(x), dt_of(x), ldx, M, ptr(w), K, ptr(ws), N, K, ptr(bias), ptr(out), dt_of(out), ldy,
-         ptr(work))
+    _work("i8.linear", work, _bytes("hmoe_i8_linear_work_bytes", M, N, K))
+    _run(x.device, "hmoe_i8_linear", x.data_ptr(), _dt("i8: x", x), ldx, M, w.data_ptr(), K, ws.data_ptr(), N, K,
+         None if bias is None else bias.data_ptr(), out.data_ptr(), _dt("i8: out", out), ldy, work.data_ptr())
     return out
 
 
 def mlp_work(device, M, H, I):
     """workspace of mlp for up to M rows"""
-    return torch.empty(max(int(lib().hmoe_i8_mlp_work_bytes(M, H, I)), 16), dtype=torch.uint8, device=torch.device(device))
+    return torch.empty(max(_bytes("hmoe_i8_mlp_work_bytes", M, H, I), 16), dtype=torch.uint8, device=torch.device(device))
 
 
 def mlp(x, wg, wu, wd, sg, su, sd, out, work):
     """out [M, H] = linear(h; wd, sd), h = silu(linear(x; wg, sg)) linear(x; wu, su) held in fp32 and quantised row by row;
     wg, wu int8 [I, H], wd int8 [H, I]"""
     on_device("i8.mlp", x, wg, wu, wd, sg, su, sd, out, work)
-    M, H = x.shape
-    I = wg.shape[0]
+    M, H = _two("i8: x", x)
+    I = _two("i8.mlp: wg", wg)[0]
     ldx, ldy = _rows("i8.mlp: x", x, M, H), _rows("i8.mlp: out", out, M, H)
     _mat("i8.mlp: wg", wg, I, H)
     _mat("i8.mlp: wu", wu, I, H)
@@ -113,7 +143,7 @@ def mlp(x, wg, wu, wd, sg, su, sd, out, work):
     _vec("i8.mlp: sg", sg, I)
     _vec("i8.mlp: su", su, I)
     _vec("i8.mlp: sd", sd, H)
-    _work("i8.mlp", work, lib().hmoe_i8_mlp_work_bytes(M, H, I))
-    _run(x.device, "hmoe_i8_mlp", ptr(x), dt_of(x), ldx, M, H, I, ptr(wg), ptr(wu), ptr(wd), ptr(sg), ptr(su), ptr(sd), ptr(out),
-         dt_of(out), ldy, ptr(work))
+    _work("i8.mlp", work, _bytes("hmoe_i8_mlp_work_bytes", M, H, I))
+    _run(x.device, "hmoe_i8_mlp", x.data_ptr(), _dt("i8: x", x), ldx, M, H, I, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), sg.data_ptr(),
+         su.data_ptr(), sd.data_ptr(), out.data_ptr(), _dt("i8: out", out), ldy, work.data_ptr())
     return out

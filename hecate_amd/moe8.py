@@ -17,15 +17,15 @@ import ctypes
 
 import torch
 
-from ._lib import dt_of, lib, on_device, ptr
-from .i8 import _rows, _run, _vec, _work
+from ._lib import on_device, ptr
+from .i8 import _bytes, _dt, _rows, _run, _two, _vec, _work
 
 _P3 = ctypes.c_void_p * 3
 
 
 def layer_work(device, T, H, I, E, topk):
     """workspace of layer for up to T tokens"""
-    nbytes = int(lib().hmoe_moe8_work_bytes(T, H, I, E, topk))
+    nbytes = _bytes("hmoe_moe8_work_bytes", T, H, I, E, topk)
     if nbytes == 0:
         raise RuntimeError(f"moe8.layer_work: {T} tokens, H {H}, I {I}, {topk} of {E} experts: not a layer this operator takes")
     return torch.empty(nbytes, dtype=torch.uint8, device=torch.device(device))
@@ -39,10 +39,12 @@ def _w(what, t, shape, dtype):
 def layer(x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, scale, lo=0, shared=None):
     """one layer of x [T, H] (bf16, fp16 or fp32) into sel int64 [T, topk], rw fp32 [T, topk] and out [T, H]"""
     on_device("moe8.layer", x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, *(shared or ()))
-    T, H = x.shape
-    E = wr.shape[0]
+    T, H = _two("moe8.layer: x", x)
+    E = _two("moe8.layer: wr", wr)[0]
+    if wg.dim() != 3:
+        raise RuntimeError(f"moe8.layer: wg must be [n, I, H], got {tuple(wg.shape)}")
     n, I = wg.shape[0], wg.shape[1]
-    topk = sel.shape[1]
+    topk = _two("moe8.layer: sel", sel)[1]
     ldx, ldy = _rows("moe8.layer: x", x, T, H), _rows("moe8.layer: out", out, T, H)
     i8, f32 = torch.int8, torch.float32
     for what, t, shape, dtype in (("wr", wr, (E, H), f32), ("wg", wg, (n, I, H), i8), ("wu", wu, (n, I, H), i8), ("wd", wd, (n, H, I), i8),
@@ -58,7 +60,8 @@ def layer(x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, scale, lo=0, 
             _w(what, t, shape, dtype)
         sw, ss = _P3(*map(ptr, shared[:3])), _P3(*map(ptr, shared[3:]))
     if T:
-        _work("moe8.layer", work, lib().hmoe_moe8_work_bytes(T, H, I, E, topk))
-    _run(x.device, "hmoe_moe8_layer", ptr(x), dt_of(x), ldx, T, ptr(wr), ptr(bias), E, topk, float(scale), ptr(wg), ptr(wu), ptr(wd),
-         ptr(sg), ptr(su), ptr(sd), n, int(lo), H, I, sw, ss, ptr(sel), ptr(rw), ptr(out), dt_of(out), ldy, ptr(work))
+        _work("moe8.layer", work, _bytes("hmoe_moe8_work_bytes", T, H, I, E, topk))
+    _run(x.device, "hmoe_moe8_layer", ptr(x), _dt("moe8.layer: x", x), ldx, T, ptr(wr), ptr(bias), E, topk, float(scale), ptr(wg), ptr(wu),
+         ptr(wd), ptr(sg), ptr(su), ptr(sd), n, int(lo), H, I, sw, ss, ptr(sel), ptr(rw), ptr(out), _dt("moe8.layer: out", out), ldy,
+         ptr(work))
     return out
