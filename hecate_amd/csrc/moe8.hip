@@ -1,11 +1,11 @@
-// moe8.hip - a whole mixture-of-experts layer for up to 16 tokens, its experts in 8 bits (hmoe_moe8_layer): scores and
-// selection, then for each distinct selected expert that is resident (and the shared expert) the gated MLP of i8.hip on the
-// tokens that chose it, joined with the routing weights.
+// moe8.hip - a whole mixture-of-experts layer for up to 16 tokens, its experts in 8 bits (hmoe_moe8_layer), in two launches:
+// the scores and the tokens in 8 bits; then the selection, and for each distinct selected expert that is resident (and the
+// shared expert) the gated MLP of i8.hip on the tokens that chose it, joined with the routing weights.
 #include "i8_dev.h"
 
 namespace hmoe {
 
-constexpr int M8_T = 16, M8_K = 16, M8_E = 512, M8_SIZE = 8192;       // tokens, picks, experts, hidden / intermediate size
+constexpr int M8_T = 16, M8_K = 16, M8_E = 512, M8_H = 7168, M8_I = 4096;      // tokens, picks, experts, hidden and intermediate size
 constexpr int M8_SLOTS = M8_T * M8_K + 1;                             // distinct experts of a call, the shared one first
 constexpr int M8_ROWS = M8_T * (M8_K + 1);                            // (expert, token) rows of a call
 
@@ -23,7 +23,7 @@ struct M8Args
     int8_t* xq; float* xs;          // [T][up128(H)], [T]
     float* act;                     // [rows][I]: silu(gate) up
     int8_t* qa; float* sa;          // [rows][up128(I)], [rows]
-    int* nrows;
+    int* ticket; int* count; int* flag;       // the next ticket; of each slot: gate/up tiles done, rows quantised
 };
 
 // ---- scores: one workgroup an expert, sums in 64 bits (scores next to each other decide the selection); behind them one
@@ -38,6 +38,8 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
     if ((int) blockIdx.x >= p.E)
     {
         const int row = blockIdx.x - p.E;
+        if (row == 0)
+            for (int i = t; i < 1 + 2 * M8_SLOTS; i += 256) p.ticket[i] = 0;       // (ticket, count, flag: one array)
         const uint8_t* xr = x + (size_t) row * p.ldx * es;
         uint32_t m = 0;
         for (int i = t; i < p.H / 16; i += 256)
@@ -88,11 +90,9 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
     if (t < p.T) p.logits[(size_t) t * p.E + blockIdx.x] = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
 }
 
-// ---- selection: every workgroup of the launches below forms it for itself ----
+// ---- the plan: which experts run on which tokens; every workgroup of the experts' kernel forms it for itself ----
 struct M8Plan
 {
-    unsigned long long key[M8_E];
-    double score[M8_E];
     int sel[M8_T][M8_K];
     double top[M8_T][M8_K];
     int mask[M8_E];                 // tokens that chose a resident expert
@@ -101,69 +101,111 @@ struct M8Plan
     uint16_t tokens[M8_SLOTS];      // its tokens, a bit each
     uint16_t row0[M8_SLOTS + 1];    // its first row: the row of its token t is row0 + the set bits below t
     float weight[M8_ROWS];
+    uint32_t scan[8];
     int slots;
 };
 
+// a number ordered as the scores are, NaN behind everything
 __device__ inline unsigned long long order_key(double v)
 {
     const unsigned long long b = (unsigned long long) __double_as_longlong(v);
-    if (v != v) return 0ull;                                             // NaN behind everything
+    if (v != v) return 0ull;
     return (b >> 63) ? ~b : b | (1ull << 63);
 }
 
-// The topk largest score + bias of each token, equal ones in the order of their ids: an expert's place is the number of
-// experts before it, counted by the thread that has it
+// The topk largest score + bias of token r by one wave: expert e is with lane e % 64, and each round takes the largest key left
+// and of equal ones the lowest id
+__device__ inline void m8_select(const M8Args& p, M8Plan& s, int r)
+{
+    constexpr int EL = M8_E / 64;
+    const int l = threadIdx.x & 63;
+    double a[EL];
+    unsigned long long k[EL];
+    #pragma unroll
+    for (int i = 0; i < EL; ++i) a[i] = 64 * i + l < p.E ? p.logits[(size_t) r * p.E + 64 * i + l] : 0.0;
+    #pragma unroll
+    for (int i = 0; i < EL; ++i)
+    {
+        k[i] = 0ull;
+        if (64 * i >= p.E) continue;
+        a[i] = 1.0 / (1.0 + exp(-a[i]));
+        const int e = 64 * i + l;
+        if (e < p.E) k[i] = order_key(p.bias ? a[i] + (double) p.bias[e] : a[i]);
+    }
+    uint32_t gone = 0;                                                   // the lane's experts that are taken
+    for (int j = 0; j < p.topk; ++j)
+    {
+        unsigned long long bk = 0ull;
+        int be = 0x7fffffff;
+        double ba = 0.0;
+        #pragma unroll
+        for (int i = 0; i < EL; ++i)
+        {
+            const int e = 64 * i + l;
+            if (e >= p.E || ((gone >> i) & 1u) || (be != 0x7fffffff && k[i] <= bk)) continue;
+            bk = k[i]; be = e; ba = a[i];
+        }
+        const uint32_t hi = wave_ext_u32<true>((uint32_t) (bk >> 32));
+        const bool ch = (uint32_t) (bk >> 32) == hi && be != 0x7fffffff;
+        const uint32_t lo = wave_ext_u32<true>(ch ? (uint32_t) bk : 0u);
+        const bool cl = ch && (uint32_t) bk == lo;
+        const int e = (int) wave_ext_u32<false>(cl ? (uint32_t) be : 0x7fffffffu);
+        if (be == e)
+        {
+            gone |= 1u << (e >> 6);
+            s.sel[r][j] = e;
+            s.top[r][j] = ba;
+        }
+    }
+}
+
 __device__ inline void m8_plan(const M8Args& p, M8Plan& s, bool write)
 {
-    const int t = threadIdx.x, nt = blockDim.x;
-    for (int e = t; e < M8_E; e += nt) s.mask[e] = 0;
-    for (int r = 0; r < p.T; ++r)
+    const int t = threadIdx.x, l = t & 63, nw = blockDim.x / 64;
+    for (int e = t; e < M8_E; e += blockDim.x) s.mask[e] = 0;
+    for (int r = t >> 6; r < p.T; r += nw) m8_select(p, s, r);
+    __syncthreads();
+    for (int i = t; i < p.T * p.topk; i += blockDim.x)
     {
-        __syncthreads();
-        for (int e = t; e < p.E; e += nt)
-        {
-            const double a = 1.0 / (1.0 + exp(-p.logits[(size_t) r * p.E + e]));
-            s.score[e] = a;
-            s.key[e] = order_key(p.bias ? a + (double) p.bias[e] : a);
-        }
-        __syncthreads();
-        for (int e = t; e < p.E; e += nt)
-        {
-            const unsigned long long k = s.key[e];
-            int place = 0;
-            for (int f = 0; f < p.E; ++f) place += s.key[f] > k || (s.key[f] == k && f < e);
-            if (place < p.topk)
-            {
-                s.sel[r][place] = e;
-                s.top[r][place] = s.score[e];
-                const int id = e - p.lo;
-                if (id >= 0 && id < p.n) atomicOr(&s.mask[id], 1 << r);
-            }
-        }
+        const int r = i / p.topk, id = s.sel[r][i - r * p.topk] - p.lo;
+        if (id >= 0 && id < p.n) atomicOr(&s.mask[id], 1 << r);
     }
     __syncthreads();
+    // slots in the order of the ids: a running count of (experts, rows) over them
+    const int m = t < M8_E ? s.mask[t] : 0;
+    uint32_t c = t < M8_E ? ((m != 0 ? 1u : 0u) << 16) + (uint32_t) __popc(m) : 0u;
+    const uint32_t own = c;
+    for (int o = 1; o < 64; o <<= 1)
+    {
+        const uint32_t v = __shfl_up(c, o);
+        c += l >= o ? v : 0u;
+    }
+    if (l == 63 && t < M8_E) s.scan[t >> 6] = c;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    #pragma unroll
+    for (int i = 0; i < M8_E / 64; ++i)
+    {
+        before += i < (t >> 6) ? s.scan[i] : 0u;
+        all += s.scan[i];
+    }
+    const int s0 = p.hg ? 1 : 0, r0 = p.hg ? p.T : 0;
+    if (t < M8_E && m)
+    {
+        const uint32_t at = before + c - own;
+        const int sl = s0 + (int) (at >> 16);
+        s.expert[sl] = (uint16_t) t; s.tokens[sl] = (uint16_t) m; s.row0[sl] = (uint16_t) (r0 + (int) (at & 0xffffu));
+        s.slot_of[t] = (uint16_t) sl;
+    }
     if (t == 0)
     {
-        int m = 0, row = 0;
-        if (p.hg)
-        {
-            s.expert[0] = 0; s.tokens[0] = (uint16_t) ((1u << p.T) - 1u); s.row0[0] = 0;
-            for (int r = 0; r < p.T; ++r) s.weight[r] = 1.0f;
-            m = 1; row = p.T;
-        }
-        for (int id = 0; id < p.n; ++id)
-            if (s.mask[id])
-            {
-                s.expert[m] = (uint16_t) id; s.tokens[m] = (uint16_t) s.mask[id]; s.row0[m] = (uint16_t) row;
-                s.slot_of[id] = (uint16_t) m;
-                row += __popc(s.mask[id]);
-                ++m;
-            }
-        s.row0[m] = (uint16_t) row;
-        s.slots = m;
+        s.slots = s0 + (int) (all >> 16);
+        s.row0[s.slots] = (uint16_t) (r0 + (int) (all & 0xffffu));
+        if (p.hg) { s.expert[0] = 0; s.tokens[0] = (uint16_t) ((1u << p.T) - 1u); s.row0[0] = 0; }
     }
+    if (p.hg && t < p.T) s.weight[t] = 1.0f;
     __syncthreads();
-    for (int i = t; i < p.T * p.topk; i += nt)
+    for (int i = t; i < p.T * p.topk; i += blockDim.x)
     {
         const int r = i / p.topk, j = i - r * p.topk, e = s.sel[r][j], id = e - p.lo;
         double sum = 0.0;
@@ -179,138 +221,377 @@ __device__ inline void m8_plan(const M8Args& p, M8Plan& s, bool write)
     __syncthreads();
 }
 
-// the sum over the 8 lanes of a group, in each of them
+// the sum over the 8 lanes of a group, in each of them. v comes out of integer dot products, whose result another instruction
+// may read three wait states later at the earliest: where the two ended up in different blocks the compiler left two (the last
+// product was missing from the sum), so the wait is written out
 __device__ __forceinline__ int sum8(int v)
 {
+    asm volatile("s_nop 2" : "+v"(v));
     v += __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);     // quad_perm [1,0,3,2]
     v += __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);     // quad_perm [2,3,0,1]
     v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);    // row_half_mirror
     return v;
 }
 
-// ---- gate and up: tile = 8 gated values of one expert ----
-__global__ void __launch_bounds__(512) m8_gate_up_kernel(M8Args p)
+// ---- the experts, gate and up to the weighted sum, in one launch ----
+// One workgroup a CU: 8 waves that stream weights, one that finishes what they sum and one that brings what they need next. The
+// work is a list of tickets, taken in order through one counter: first the gate/up tiles (8 TR gated values of one expert: slot
+// after slot, the shared expert first), then the down tiles (8 output columns, over every slot, a batch of slots at a time).
+//
+// A slot's last gate/up tile (by a count) quantises its rows and raises its flag; a down batch waits for its slots' flags. Those
+// come from earlier tickets alone, which are held by workgroups that run already; a workgroup waits for no flag before all its
+// gate/up tiles are counted. So every wait ends, whatever else is on the card and however many of this launch's workgroups have
+// started (all the same it is bounded: past the bound the output is NaN).
+//
+// Weights are read 8 rows x 128 bytes a load, each wave its own slice of the depth, one item (12 loads of 1 KB or so a wave)
+// ahead, and multiplied by 4-wide integer dot products with the tokens' values out of LDS: an expert has one or two tokens of a
+// step, for which a matrix instruction would be mostly empty, and whole lines arrive faster from memory than a matrix
+// fragment's order (16 rows x 64 bytes): 7.0 against 5.7 TB/s over 3.2 GB. The streaming waves load nothing else: loads return
+// in order, so whatever they waited for would wait for the weights in flight.
+//
+// A wave's whole numbers are exact; those of a down tile are scaled and added slot by slot in fp32, then over the 8 waves: the
+// same order every time.
+constexpr int M8_ARENA = 140 * 1024, M8_RQ = 32;                        // LDS of x, partial sums and quantised rows; rows of a batch
+
+template <int NS, int TR, int NSD>
+__global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
 {
+    constexpr int NG2 = 2 * NS * TR, SB = NG2 / NSD < 6 ? (NG2 / NSD > 0 ? NG2 / NSD : 1) : 6;     // slots of a batch
+    constexpr int NL = NG2 > SB * NSD ? NG2 : SB * NSD;                 // loads of an item
+    constexpr int XP = 1024 * NS, ROWS = 16 * TR;                       // LDS row of x; rows of a gate/up tile
+    static_assert(M8_T * (XP + 64 * ROWS) <= M8_ARENA && 2 * M8_T * 1024 * NSD <= M8_ARENA, "LDS");
     __shared__ M8Plan s;
-    __shared__ int red[8][2][8][M8_T];
-    m8_plan(p, s, blockIdx.x == 0);
-    const int t = threadIdx.x, l = t & 63, w = t >> 6, r = l >> 3, pc = l & 7;
-    if (blockIdx.x == 0 && t == 0) *p.nrows = s.row0[s.slots];
-    const int NB = cdiv(p.I, 8), NC = cdiv(p.H, 128);
-    for (int tile = blockIdx.x; tile < s.slots * NB; tile += gridDim.x)
+    __shared__ __attribute__((aligned(16))) int8_t arena[M8_ARENA];
+    __shared__ float accl[2][8][8][M8_T];
+    __shared__ float fq[2][M8_RQ];
+    __shared__ uint16_t bst[M8_SLOTS + 1];                              // first slot of each batch
+    __shared__ int tk[4], nbl;
+    const int t = threadIdx.x, l = t & 63, r = l >> 3, pc = l & 7;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    constexpr int QP = 1024 * NSD;                                      // LDS row of a batch
+    const int T = p.T, IP = (int) up128(p.I), HP = (int) up128(p.H);
+    // x [T][XP], partial sums [2][8][ROWS][T] and the batches' rows [2][rq][QP]: side by side, or the rows in the others' place
+    int8_t* xl = arena;
+    int* red = (int*) (arena + T * XP);
+    const int xr_bytes = T * (XP + 64 * ROWS);
+    const bool apart = xr_bytes + 2 * T * QP <= M8_ARENA;
+    int8_t* qb = apart ? arena + xr_bytes : arena;
+    const int rq = min((M8_ARENA - (apart ? xr_bytes : 0)) / (2 * QP), M8_RQ);
+    if (t == 0)
     {
-        const int sl = tile / NB, n0 = 8 * (tile - sl * NB), n = min(n0 + r, p.I - 1);
-        const bool sh = p.hg && sl == 0;
-        const size_t wo = (sh ? 0 : (size_t) s.expert[sl] * p.I * p.H) + (size_t) n * p.H;
-        const int8_t* wg = (sh ? p.hg : p.wg) + wo;
-        const int8_t* wu = (sh ? p.hu : p.wu) + wo;
-        int k = 0;
-        for (uint32_t m = s.tokens[sl]; m; m &= m - 1, ++k)
-        {
-            const int8_t* xr = p.xq + (size_t) __builtin_ctz(m) * up128(p.H);
-            int ag = 0, au = 0;
-            for (int c = w; c < NC; c += 8)
+        const int v = __hip_atomic_fetch_add(p.ticket, 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        tk[0] = v; tk[1] = v + 1;
+    }
+    for (int i = t; i < T * (XP / 16); i += 640)
+    {
+        const int tok = i / (XP / 16), k = 16 * (i - tok * (XP / 16));
+        *(u32x4*) (xl + tok * XP + k) = k < p.H ? ld16(p.xq + (size_t) tok * HP + k) : (u32x4) {0u, 0u, 0u, 0u};
+    }
+    m8_plan(p, s, blockIdx.x == 0);
+    const int slots = s.slots, NB = cdiv(p.I, 8 * TR), NG = slots * NB, total = NG + cdiv(p.H, 8);
+    if (t == 0)
+    {
+        int n = 0, first = 0;
+        for (int sl = 0; sl < slots; ++sl)
+            if (sl == 0 || sl - first == SB || s.row0[sl + 1] - s.row0[first] > rq) { bst[n++] = (uint16_t) sl; first = sl; }
+        bst[n] = (uint16_t) slots;
+        nbl = n;
+    }
+    __syncthreads();
+    const int nb = max(nbl, 1);                                         // batches of a down tile
+
+    // an item: a gate/up tile (batch < 0) or one batch of a down tile; d counts the down items
+    struct Item { int ticket, seq, slot, blk, batch, d; };
+    auto item = [&](int ticket, int seq, int d) {
+        Item it = {ticket, seq, 0, 0, -1, d};
+        if (ticket < NG) { it.slot = ticket / NB; it.blk = ticket - it.slot * NB; }
+        else { it.blk = ticket - NG; it.batch = 0; ++it.d; }
+        return it;
+    };
+    auto next = [&](const Item& c) {
+        if (c.batch >= 0 && c.batch + 1 < nb) { Item it = c; ++it.batch; ++it.d; return it; }
+        return item(__builtin_amdgcn_readfirstlane(tk[(c.seq + 1) & 3]), c.seq + 1, c.d);
+    };
+    // between the last gate/up tile and the first down batch: what is brought then may wait for this workgroup's own tiles
+    auto turns = [&](const Item& c, const Item& n) { return c.batch < 0 && n.batch >= 0 && n.ticket < total; };
+    Item cur = item(__builtin_amdgcn_readfirstlane(tk[0]), 0, 0);
+
+    if (w == 9)
+    {
+        // the bringing wave: tickets, and the rows of the next down batch
+        int ready = 0;                                                   // slots below it are known to be quantised
+        bool lost = false;
+        auto bring = [&](const Item& it) {
+            if (it.batch < 0 || it.ticket >= total || slots == 0) return;
+            const int s0 = bst[it.batch], s1 = bst[it.batch + 1], r0 = s.row0[s0], n = s.row0[s1] - r0;
+            for (int polls = 0; ready < s1 && !lost; ++polls)
             {
-                const int off = 128 * c + 16 * pc;
-                if (off < p.H)
+                const int f = ready + l;
+                const int v = f < slots ? __hip_atomic_load(p.flag + f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+                const unsigned long long up = __ballot(v != 0);
+                ready += up == ~0ull ? 64 : __builtin_ctzll(~up);
+                if (ready < s1) __builtin_amdgcn_s_sleep(4);
+                lost = polls > (1 << 22);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            int8_t* q = qb + (it.d & 1) * rq * QP;
+            #pragma unroll 8
+            for (int i = l; i < n * (QP / 16); i += 64)
+            {
+                const int row = i / (QP / 16), k = 16 * (i % (QP / 16));
+                *(u32x4*) (q + 16 * i) = k < p.I ? ld16(p.qa + (size_t) (r0 + row) * IP + k) : (u32x4) {0u, 0u, 0u, 0u};
+            }
+            if (l < n) fq[it.d & 1][l] = lost ? __uint_as_float(0x7fc00000u) : p.sa[r0 + l] * s.weight[r0 + l];
+        };
+        bring(cur);
+        __syncthreads();
+        while (cur.ticket < total)
+        {
+            const bool fetch = cur.batch <= 0;                           // the ticket after the next: one a ticket
+            int nt = 0;
+            if (fetch && l == 0) nt = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const Item nx = next(cur);
+            const bool turn = turns(cur, nx);
+            if (!turn) bring(nx);
+            if (fetch && l == 0) tk[(cur.seq + 2) & 3] = nt;
+            __syncthreads();
+            if (turn)
+            {
+                if (!apart) __syncthreads();
+                bring(nx);
+                __syncthreads();
+            }
+            cur = nx;
+        }
+        return;
+    }
+    if (w == 8)
+    {
+        // the finishing wave
+        __syncthreads();
+        while (cur.ticket < total)
+        {
+            const bool gu = cur.batch < 0, sh = p.hg && cur.slot == 0;
+            float sg = 0.f, su = 0.f;
+            if (gu && l < 8 * TR)
+            {
+                const size_t so = (sh ? 0 : (size_t) s.expert[cur.slot] * p.I) + min(8 * TR * cur.blk + l, p.I - 1);
+                sg = (sh ? p.hsg : p.sg)[so];
+                su = (sh ? p.hsu : p.su)[so];
+            }
+            const Item nx = next(cur);
+            __syncthreads();
+            if (gu)
+            {
+                const uint32_t mask = s.tokens[cur.slot];
+                const int m = __popc(mask), row0 = s.row0[cur.slot];
+                const int* rd = red + (cur.seq & 1) * 8 * ROWS * T;
+                for (int i0 = 0; i0 < 8 * TR * m; i0 += 64)
                 {
-                    const u32x4 xv = ld16(xr + off);
-                    ag = dot16(ld16(wg + off), xv, ag);
-                    au = dot16(ld16(wu + off), xv, au);
+                    const int i = min(i0 + l, 8 * TR * m - 1), k = i / (8 * TR), rr = i - k * 8 * TR, n = 8 * TR * cur.blk + rr;
+                    int ag = 0, au = 0;
+                    #pragma unroll
+                    for (int v = 0; v < 8; ++v)
+                    {
+                        ag += rd[(v * ROWS + rr) * T + k];
+                        au += rd[(v * ROWS + 8 * TR + rr) * T + k];
+                    }
+                    uint32_t mm = mask;
+                    for (int j = 0; j < k; ++j) mm &= mm - 1;
+                    const float xs = p.xs[__builtin_ctz(mm)];
+                    const float g = (float) ag * xs * __shfl(sg, rr), u = (float) au * xs * __shfl(su, rr);
+                    if (i0 + l < 8 * TR * m && n < p.I)
+                        __hip_atomic_store(p.act + (size_t) (row0 + k) * p.I + n, swiglu(g, u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+                int done = 0;
+                if (l == 0) done = __hip_atomic_fetch_add(p.count + cur.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (__builtin_amdgcn_readfirstlane(done) == NB - 1)
+                {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+                    for (int k = 0; k < m; ++k)
+                    {
+                        const float* a = p.act + (size_t) (row0 + k) * p.I;
+                        uint32_t top = 0;
+                        for (int i = l; i < p.I / 16; i += 64)
+                        {
+                            float v[16];
+                            load16<HMOE_DT_F32, true>(a, i, v);
+                            #pragma unroll
+                            for (int j = 0; j < 16; ++j) top = max(top, mag(v[j]));
+                        }
+                        const RowQ q = row_q(wave_ext_u32<true>(top));
+                        for (int i = l; i < p.I / 16; i += 64)
+                        {
+                            float v[16];
+                            load16<HMOE_DT_F32, true>(a, i, v);
+                            *(u32x4*) (p.qa + (size_t) (row0 + k) * IP + 16 * i) = quant16<HMOE_DT_BF16>(v, q);
+                        }
+                        if (l == 0) p.sa[row0 + k] = q.s;
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+                    if (l == 0) __hip_atomic_store(p.flag + cur.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
             }
-            ag = sum8(ag); au = sum8(au);
-            if (pc == 0) { red[w][0][r][k] = ag; red[w][1][r][k] = au; }
-        }
-        __syncthreads();
-        if (t < 8 * k)
-        {
-            const int rr = t & 7, kk = t >> 3, nn = n0 + rr;
-            if (nn < p.I)
+            else if (cur.batch + 1 == nb)
             {
-                int ag = 0, au = 0;
-                for (int v = 0; v < 8; ++v) { ag += red[v][0][rr][kk]; au += red[v][1][rr][kk]; }
-                uint32_t m = s.tokens[sl];
-                for (int i = 0; i < kk; ++i) m &= m - 1;
-                const float xs = p.xs[__builtin_ctz(m)];
-                const size_t so = (sh ? 0 : (size_t) s.expert[sl] * p.I) + nn;
-                const float g = (float) ag * xs * (sh ? p.hsg : p.sg)[so], u = (float) au * xs * (sh ? p.hsu : p.su)[so];
-                p.act[(size_t) (s.row0[sl] + kk) * p.I + nn] = swiglu(g, u);
+                for (int i = l; i < 8 * T; i += 64)
+                {
+                    const int rr = i & 7, tok = i >> 3;
+                    float v = 0.f;
+                    #pragma unroll
+                    for (int k = 0; k < 8; ++k) v += accl[cur.seq & 1][k][rr][tok];
+                    if (8 * cur.blk + rr < p.H) store_out(p.y, (size_t) tok * p.ldy + 8 * cur.blk + rr, v, p.ydt);
+                }
+            }
+            if (turns(cur, nx))
+            {
+                if (!apart) __syncthreads();
+                __syncthreads();
+            }
+            cur = nx;
+        }
+        return;
+    }
+
+    // a streaming wave: its slice of the depth is NS (gate, up) or NSD (down) lines of 128 bytes from line w NS (w NSD) on; a
+    // piece behind the depth re-reads the row's last 16 bytes, against values that are taken as zero
+    u32x4 a[2][NL];
+    float sd[2][SB];
+    auto load = [&](const Item& it, u32x4 (&d)[NL], float (&sc)[SB]) {
+        if (it.ticket >= total) return;
+        if (it.batch < 0)
+        {
+            const bool sh = p.hg && it.slot == 0;
+            const size_t eo = sh ? 0 : (size_t) s.expert[it.slot] * p.I * p.H;
+            const int8_t* wg = (sh ? p.hg : p.wg) + eo;
+            const int8_t* wu = (sh ? p.hu : p.wu) + eo;
+            #pragma unroll
+            for (int tr = 0; tr < TR; ++tr)
+            {
+                const size_t ro = (size_t) min(8 * (TR * it.blk + tr) + r, p.I - 1) * p.H;
+                #pragma unroll
+                for (int i = 0; i < NS; ++i)
+                {
+                    const int off = min(128 * (w * NS + i) + 16 * pc, p.H - 16);
+                    d[tr * NS + i] = ldw16(wg + ro + off);
+                    d[(TR + tr) * NS + i] = ldw16(wu + ro + off);
+                }
             }
         }
-        __syncthreads();
-    }
-}
-
-__global__ void __launch_bounds__(256) m8_quant_kernel(M8Args p)
-{
-    __shared__ uint32_t wmax[4];
-    const int t = threadIdx.x, row = blockIdx.x;
-    if (row >= *p.nrows) return;
-    const float* a = p.act + (size_t) row * p.I;
-    uint32_t m = 0;
-    for (int i = t; i < p.I; i += 256) m = max(m, mag(a[i]));
-    m = wave_ext_u32<true>(m);
-    if ((t & 63) == 0) wmax[t >> 6] = m;
-    __syncthreads();
-    const RowQ q = row_q(max(max(wmax[0], wmax[1]), max(wmax[2], wmax[3])));
-    if (t == 0) p.sa[row] = q.s;
-    for (int i = t; i < p.I / 16; i += 256)
-    {
-        float v[16];
-        load16<HMOE_DT_F32, true>(a, i, v);
-        *(u32x4*) (p.qa + (size_t) row * up128(p.I) + 16 * i) = quant16<HMOE_DT_F32>(v, q);
-    }
-}
-
-// ---- down: tile = 8 output columns, over every expert in the order of its slot ----
-__global__ void __launch_bounds__(512) m8_down_kernel(M8Args p)
-{
-    __shared__ M8Plan s;
-    __shared__ float acc[8][8][M8_T];
-    m8_plan(p, s, false);
-    const int t = threadIdx.x, l = t & 63, w = t >> 6, r = l >> 3, pc = l & 7;
-    const int NB = cdiv(p.H, 8), NC = cdiv(p.I, 128);
-    for (int tile = blockIdx.x; tile < NB; tile += gridDim.x)
-    {
-        const int n0 = 8 * tile, n = min(n0 + r, p.H - 1);
-        for (int i = t; i < 8 * 8 * M8_T; i += 512) (&acc[0][0][0])[i] = 0.f;
-        __syncthreads();
-        for (int sl = 0; sl < s.slots; ++sl)
+        else if (slots > 0)
         {
-            const bool sh = p.hg && sl == 0;
-            const int8_t* wd = (sh ? p.hd : p.wd + (size_t) s.expert[sl] * p.H * p.I) + (size_t) n * p.I;
-            const float sd = (sh ? p.hsd : p.sd + (size_t) s.expert[sl] * p.H)[n];
-            int row = s.row0[sl];
+            const int n = min(8 * it.blk + r, p.H - 1), s0 = bst[it.batch], s1 = bst[it.batch + 1];
+            #pragma unroll
+            for (int b = 0; b < SB; ++b)
+            {
+                const int sl = s0 + b;
+                if (sl >= s1) break;
+                const bool sh = p.hg && sl == 0;
+                const int8_t* wd = (sh ? p.hd : p.wd + (size_t) s.expert[sl] * p.H * p.I) + (size_t) n * p.I;
+                #pragma unroll
+                for (int i = 0; i < NSD; ++i) d[b * NSD + i] = ldw16(wd + min(128 * (w * NSD + i) + 16 * pc, p.I - 16));
+                sc[b] = (sh ? p.hsd : p.sd + (size_t) s.expert[sl] * p.H)[n];
+            }
+        }
+    };
+    auto compute = [&](const Item& it, const u32x4 (&d)[NL], const float (&sc)[SB]) {
+        if (it.batch < 0)
+        {
+            int* rd = red + ((it.seq & 1) * 8 + w) * ROWS * T;
+            int k = 0;
+            for (uint32_t m = s.tokens[it.slot]; m; m &= m - 1, ++k)
+            {
+                const int8_t* x = xl + __builtin_ctz(m) * XP + 128 * w * NS + 16 * pc;
+                int g[TR], u[TR];
+                #pragma unroll
+                for (int tr = 0; tr < TR; ++tr) g[tr] = u[tr] = 0;
+                #pragma unroll
+                for (int i = 0; i < NS; ++i)
+                {
+                    const u32x4 xv = *(const u32x4*) (x + 128 * i);
+                    #pragma unroll
+                    for (int tr = 0; tr < TR; ++tr)
+                    {
+                        g[tr] = dot16(d[tr * NS + i], xv, g[tr]);
+                        u[tr] = dot16(d[(TR + tr) * NS + i], xv, u[tr]);
+                    }
+                }
+                #pragma unroll
+                for (int tr = 0; tr < TR; ++tr)
+                {
+                    const int gs = sum8(g[tr]), us = sum8(u[tr]);
+                    if (pc == 0)
+                    {
+                        rd[(8 * tr + r) * T + k] = gs;
+                        rd[(8 * (TR + tr) + r) * T + k] = us;
+                    }
+                }
+            }
+            return;
+        }
+        float (*acc)[M8_T] = accl[it.seq & 1][w];
+        if (it.batch == 0)
+            for (int i = l; i < 8 * M8_T; i += 64) (&acc[0][0])[i] = 0.f;
+        if (slots == 0) return;
+        const int s0 = bst[it.batch], s1 = bst[it.batch + 1], r0 = s.row0[s0];
+        const int8_t* qr = qb + (it.d & 1) * rq * QP + 128 * w * NSD + 16 * pc;
+        const float* f = fq[it.d & 1];
+        #pragma unroll
+        for (int b = 0; b < SB; ++b)
+        {
+            const int sl = s0 + b;
+            if (sl >= s1) break;
+            int row = s.row0[sl] - r0;
             for (uint32_t m = s.tokens[sl]; m; m &= m - 1, ++row)
             {
-                int a = 0;
-                for (int c = w; c < NC; c += 8)
-                {
-                    const int off = 128 * c + 16 * pc;
-                    if (off < p.I) a = dot16(ld16(wd + off), ld16(p.qa + (size_t) row * up128(p.I) + off), a);
-                }
-                a = sum8(a);
-                if (pc == 0) acc[w][r][__builtin_ctz(m)] += (float) a * (p.sa[row] * sd) * s.weight[row];
+                int v = 0;
+                #pragma unroll
+                for (int i = 0; i < NSD; ++i) v = dot16(d[b * NSD + i], *(const u32x4*) (qr + row * QP + 128 * i), v);
+                v = sum8(v);
+                if (pc == 0) acc[r][__builtin_ctz(m)] += (float) v * (f[row] * sc[b]);
             }
         }
+    };
+    auto turn = [&](const Item& c, const Item& n) {
+        if (!turns(c, n)) return;
+        if (!apart) __syncthreads();
         __syncthreads();
-        if (t < 8 * p.T)
-        {
-            const int rr = t & 7, tk = t >> 3;
-            float v = 0.f;
-            for (int k = 0; k < 8; ++k) v += acc[k][rr][tk];
-            if (n0 + rr < p.H) store_out(p.y, (size_t) tk * p.ldy + n0 + rr, v, p.ydt);
-        }
+    };
+    load(cur, a[0], sd[0]);
+    __syncthreads();
+    while (cur.ticket < total)
+    {
+        Item nx = next(cur);
+        load(nx, a[1], sd[1]);
+        compute(cur, a[0], sd[0]);
         __syncthreads();
+        turn(cur, nx);
+        cur = nx;
+        if (cur.ticket >= total) break;
+        nx = next(cur);
+        load(nx, a[0], sd[0]);
+        compute(cur, a[1], sd[1]);
+        __syncthreads();
+        turn(cur, nx);
+        cur = nx;
     }
+}
+
+template <int NS, int TR>
+static void m8_launch(const M8Args& p, hipStream_t st)
+{
+    if (p.I <= 1024) m8_experts_kernel<NS, TR, 1><<<256, 640, 0, st>>>(p);
+    else if (p.I <= 2048) m8_experts_kernel<NS, TR, 2><<<256, 640, 0, st>>>(p);
+    else m8_experts_kernel<NS, TR, 4><<<256, 640, 0, st>>>(p);
 }
 
 // workspace layout; the parts' offsets into o (or null) and the whole size
 static size_t m8_layout(int T, int H, int I, int E, int topk, size_t* o)
 {
     const size_t rows = (size_t) T * (topk + 1);
-    const size_t part[] = {(size_t) T * E * 8, (size_t) T * up128(H), (size_t) T * 4, rows * I * 4, rows * up128(I), rows * 4, 128};
+    const size_t part[] = {(size_t) T * E * 8, (size_t) T * up128(H), (size_t) T * 4, rows * I * 4, rows * up128(I), rows * 4,
+                           (1 + 2 * M8_SLOTS) * 4};
     size_t at = 0;
     for (int i = 0; i < 7; ++i)
     {
@@ -326,7 +607,7 @@ using namespace hmoe;
 
 extern "C" size_t hmoe_moe8_work_bytes(int T, int H, int I, int E, int topk)
 {
-    if (T < 1 || T > M8_T || H < 16 || H > M8_SIZE || I < 16 || I > M8_SIZE || E < 1 || E > M8_E || topk < 1 || topk > M8_K) return 0;
+    if (T < 1 || T > M8_T || H < 16 || H > M8_H || I < 16 || I > M8_I || E < 1 || E > M8_E || topk < 1 || topk > M8_K) return 0;
     return m8_layout(T, H, I, E, topk, nullptr);
 }
 
@@ -339,8 +620,8 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
     const auto dt_ok = [](int d) { return d == HMOE_DT_F32 || d == HMOE_DT_BF16 || d == HMOE_DT_F16; };
     const auto at = [](const void* q, int a) { return q && ((uintptr_t) q & (a - 1)) == 0; };
     HMOE_REQUIRE(T > 0 && T <= M8_T, "moe8_layer: %d tokens: up to %d", T, M8_T);
-    HMOE_REQUIRE(H >= 16 && H <= M8_SIZE && H % 16 == 0 && I >= 16 && I <= M8_SIZE && I % 16 == 0,
-                 "moe8_layer: hidden size %d, intermediate size %d: multiples of 16 up to %d", H, I, M8_SIZE);
+    HMOE_REQUIRE(H >= 16 && H <= M8_H && H % 16 == 0 && I >= 16 && I <= M8_I && I % 16 == 0,
+                 "moe8_layer: hidden size %d, intermediate size %d: multiples of 16 up to %d and %d", H, I, M8_H, M8_I);
     HMOE_REQUIRE(E >= 1 && E <= M8_E && topk >= 1 && topk <= M8_K && topk <= E, "moe8_layer: %d of %d experts: up to %d of %d", topk, E,
                  M8_K, M8_E);
     HMOE_REQUIRE(n >= 0 && lo >= 0 && lo <= E - n, "moe8_layer: resident experts [%d, %d + %d) of %d", lo, lo, n, E);
@@ -367,7 +648,7 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
                 sh_s ? sh_s[0] : nullptr, sh_s ? sh_s[1] : nullptr, sh_s ? sh_s[2] : nullptr,
                 T, H, I, E, n, lo, topk, scale, sel, rw, y, ldy, y_dtype,
                 (double*) (b + o[0]), (int8_t*) (b + o[1]), (float*) (b + o[2]), (float*) (b + o[3]), (int8_t*) (b + o[4]),
-                (float*) (b + o[5]), (int*) (b + o[6])};
+                (float*) (b + o[5]), (int*) (b + o[6]), (int*) (b + o[6]) + 1, (int*) (b + o[6]) + 1 + M8_SLOTS};
     const hipStream_t st = (hipStream_t) stream;
     const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * (x_dtype == HMOE_DT_F32 ? 4 : 2)) % 16 == 0;
 #define HMOE_R(D, V) m8_route_kernel<D, V><<<E + T, 256, 0, st>>>(p)
@@ -375,8 +656,11 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
     else if (x_dtype == HMOE_DT_BF16) { if (vec) HMOE_R(HMOE_DT_BF16, true); else HMOE_R(HMOE_DT_BF16, false); }
     else { if (vec) HMOE_R(HMOE_DT_F16, true); else HMOE_R(HMOE_DT_F16, false); }
 #undef HMOE_R
-    m8_gate_up_kernel<<<1024, 512, 0, st>>>(p);
-    m8_quant_kernel<<<T * (topk + 1), 256, 0, st>>>(p);
-    m8_down_kernel<<<cdiv(H, 8), 512, 0, st>>>(p);
+    // the lines of a hidden row that a wave takes, and as many 8-row groups as make 8 to 14 loads of an item with them
+    if (H <= 1024) m8_launch<1, 6>(p, st);
+    else if (H <= 2048) m8_launch<2, 3>(p, st);
+    else if (H <= 4096) m8_launch<4, 1>(p, st);
+    else if (H <= 6144) m8_launch<6, 1>(p, st);
+    else m8_launch<7, 1>(p, st);
     return HMOE_LAUNCHED("moe8 layer");
 }

@@ -278,7 +278,7 @@ int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H, int I, co
  * runtime/core/exl3_router.py:94-127). y [T][H] = the sum over the selected experts with lo <= id < lo + n of rw times
  * their gated MLP (wg, wu [n][I][H], wd [n][H][I], scales [n][I], [n][I], [n][H]) and the shared expert's (sh_w / sh_s, host
  * arrays of three device addresses, gate, up, down; both NULL without one). T <= 16, topk <= 16, E <= 512, H and I multiples
- * of 16 up to 8192. wr and the weights are 16-byte aligned, the workspace (hmoe_moe8_work_bytes, 0 for sizes that are refused)
+ * of 16 up to 7168 and 4096. wr and the weights are 16-byte aligned, the workspace (hmoe_moe8_work_bytes, 0 for sizes that are refused)
  * 128-byte; a workspace made for more tokens serves fewer. T = 0 is a no-op. y overlaps no input. ---- */
 size_t hmoe_moe8_work_bytes(int T, int H, int I, int E, int topk);
 int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, const float* wr, const float* bias, int E, int topk, double scale,

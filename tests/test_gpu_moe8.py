@@ -101,7 +101,7 @@ def rows(T, H, dtype, seed, dev, pad=0):
 SIZES = [  # E, n, lo, H, I, topk, shared
     (1, 1, 0, 16, 16, 1, False), (3, 3, 0, 48, 80, 2, True), (8, 8, 0, 256, 128, 2, True), (60, 40, 11, 512, 352, 4, False),
     (64, 1, 63, 144, 272, 6, True), (20, 20, 0, 1024, 704, 16, True), (128, 100, 0, 2048, 144, 8, False), (512, 512, 0, 96, 32, 16, True),
-    (7, 7, 0, 6144, 2048, 3, True), (4, 4, 0, 8192, 48, 4, False), (4, 4, 0, 48, 8192, 4, True), (257, 200, 57, 176, 1104, 5, True),
+    (7, 7, 0, 6144, 2048, 3, True), (4, 4, 0, 7168, 48, 4, False), (4, 4, 0, 48, 4096, 4, True), (257, 200, 57, 176, 1104, 5, True),
     (5, 5, 0, 4096, 1536, 2, True), (9, 9, 0, 7168, 208, 8, False), (6, 6, 0, 1040, 2064, 2, True)]
 
 

@@ -21,9 +21,10 @@ def test_layer_refuses():
     refused("tokens", T=17)
     refused("tokens", T=-1)
     refused("hidden size", H=72)
-    refused("hidden size", H=8208, ldx=8208, ldy=8208)
+    refused("hidden size", H=7184, ldx=7184, ldy=7184)
     refused("hidden size", I=8)
     refused("hidden size", I=0)
+    refused("hidden size", I=4112)
     refused("experts", E=513)
     refused("experts", topk=17)
     refused("experts", topk=0)
