@@ -101,6 +101,7 @@ struct M8Plan
     uint16_t tokens[M8_SLOTS];      // its tokens, a bit each
     uint16_t row0[M8_SLOTS + 1];    // its first row: the row of its token t is row0 + the set bits below t
     float weight[M8_ROWS];
+    float xs[M8_T];
     uint32_t scan[8];
     int slots;
 };
@@ -163,6 +164,7 @@ __device__ inline void m8_plan(const M8Args& p, M8Plan& s, bool write)
 {
     const int t = threadIdx.x, l = t & 63, nw = blockDim.x / 64;
     for (int e = t; e < M8_E; e += blockDim.x) s.mask[e] = 0;
+    if (t < p.T) s.xs[t] = p.xs[t];
     for (int r = t >> 6; r < p.T; r += nw) m8_select(p, s, r);
     __syncthreads();
     for (int i = t; i < p.T * p.topk; i += blockDim.x)
@@ -367,18 +369,20 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     }
     if (w == 8)
     {
-        // the finishing wave
+        // the finishing wave; the next tile's scales are on their way while it finishes one
+        float sg = 0.f, su = 0.f;
+        auto scales = [&](const Item& it) {
+            if (it.batch >= 0 || l >= 8 * TR) return;
+            const bool sh = p.hg && it.slot == 0;
+            const size_t so = (sh ? 0 : (size_t) s.expert[it.slot] * p.I) + min(8 * TR * it.blk + l, p.I - 1);
+            sg = (sh ? p.hsg : p.sg)[so];
+            su = (sh ? p.hsu : p.su)[so];
+        };
+        if (cur.ticket < total) scales(cur);
         __syncthreads();
         while (cur.ticket < total)
         {
-            const bool gu = cur.batch < 0, sh = p.hg && cur.slot == 0;
-            float sg = 0.f, su = 0.f;
-            if (gu && l < 8 * TR)
-            {
-                const size_t so = (sh ? 0 : (size_t) s.expert[cur.slot] * p.I) + min(8 * TR * cur.blk + l, p.I - 1);
-                sg = (sh ? p.hsg : p.sg)[so];
-                su = (sh ? p.hsu : p.su)[so];
-            }
+            const bool gu = cur.batch < 0;
             const Item nx = next(cur);
             __syncthreads();
             if (gu)
@@ -398,12 +402,15 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
                     }
                     uint32_t mm = mask;
                     for (int j = 0; j < k; ++j) mm &= mm - 1;
-                    const float xs = p.xs[__builtin_ctz(mm)];
+                    const float xs = s.xs[__builtin_ctz(mm)];
                     const float g = (float) ag * xs * __shfl(sg, rr), u = (float) au * xs * __shfl(su, rr);
                     if (i0 + l < 8 * TR * m && n < p.I)
                         __hip_atomic_store(p.act + (size_t) (row0 + k) * p.I + n, swiglu(g, u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+                if (nx.ticket < total) scales(nx);
+                // (the values were stored past the XCD's own L2, as stores at the agent's scope are: once they are counted off they
+                // can be seen, without writing the L2's lines back first, which takes longer than a tile)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 int done = 0;
                 if (l == 0) done = __hip_atomic_fetch_add(p.count + cur.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (__builtin_amdgcn_readfirstlane(done) == NB - 1)
