@@ -8,6 +8,7 @@ namespace hmoe {
 constexpr int M8_T = 16, M8_K = 16, M8_E = 512, M8_H = 7168, M8_I = 4096;      // tokens, picks, experts, hidden and intermediate size
 constexpr int M8_SLOTS = M8_T * M8_K + 1;                             // distinct experts of a call, the shared one first
 constexpr int M8_ROWS = M8_T * (M8_K + 1);                            // (expert, token) rows of a call
+constexpr int M8_SYNC = 32 + 33 * M8_SLOTS;                           // the ticket counter, the slots' counts (a line each) and flags
 
 struct M8Args
 {
@@ -39,7 +40,7 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
     {
         const int row = blockIdx.x - p.E;
         if (row == 0)
-            for (int i = t; i < 1 + 2 * M8_SLOTS; i += 256) p.ticket[i] = 0;       // (ticket, count, flag: one array)
+            for (int i = t; i < M8_SYNC; i += 256) p.ticket[i] = 0;                // (ticket, count, flag: one array)
         const uint8_t* xr = x + (size_t) row * p.ldx * es;
         uint32_t m = 0;
         for (int i = t; i < p.H / 16; i += 256)
@@ -121,9 +122,18 @@ __device__ inline void m8_select(const M8Args& p, M8Plan& s, int r)
     constexpr int EL = M8_E / 64;
     const int l = threadIdx.x & 63;
     double a[EL];
+    float bs[EL];
     unsigned long long k[EL];
+    // (every load asked for before any is used: a round trip each would be most of the plan's time)
     #pragma unroll
-    for (int i = 0; i < EL; ++i) a[i] = 64 * i + l < p.E ? p.logits[(size_t) r * p.E + 64 * i + l] : 0.0;
+    for (int i = 0; i < EL; ++i)
+    {
+        const int e = min(64 * i + l, p.E - 1);
+        a[i] = ldg<double>(p.logits + (size_t) r * p.E + e);
+        bs[i] = ldg<float>(p.bias ? p.bias + e : p.wr);
+    }
+    #pragma unroll
+    for (int i = 0; i < EL; ++i) asm volatile("" : "+v"(a[i]), "+v"(bs[i]));
     #pragma unroll
     for (int i = 0; i < EL; ++i)
     {
@@ -131,7 +141,7 @@ __device__ inline void m8_select(const M8Args& p, M8Plan& s, int r)
         if (64 * i >= p.E) continue;
         a[i] = 1.0 / (1.0 + exp(-a[i]));
         const int e = 64 * i + l;
-        if (e < p.E) k[i] = order_key(p.bias ? a[i] + (double) p.bias[e] : a[i]);
+        if (e < p.E) k[i] = order_key(p.bias ? a[i] + (double) bs[i] : a[i]);
     }
     uint32_t gone = 0;                                                   // the lane's experts that are taken
     for (int j = 0; j < p.topk; ++j)
@@ -164,8 +174,9 @@ __device__ inline void m8_plan(const M8Args& p, M8Plan& s, bool write)
 {
     const int t = threadIdx.x, l = t & 63, nw = blockDim.x / 64;
     for (int e = t; e < M8_E; e += blockDim.x) s.mask[e] = 0;
-    if (t < p.T) s.xs[t] = p.xs[t];
-    for (int r = t >> 6; r < p.T; r += nw) m8_select(p, s, r);
+    const int lt = t - (int) blockDim.x + 64;
+    if (lt >= 0 && lt < p.T) s.xs[lt] = p.xs[lt];                        // (the last wave too)
+    for (int r = nw - 1 - (t >> 6); r < p.T; r += nw) m8_select(p, s, r);         // (the last waves first: they stream nothing)
     __syncthreads();
     for (int i = t; i < p.T * p.topk; i += blockDim.x)
     {
@@ -235,6 +246,19 @@ __device__ __forceinline__ int sum8(int v)
     return v;
 }
 
+// an address that is the same in every lane, in scalar registers
+template <typename T> __device__ __forceinline__ const T* scalar(const T* q)
+{
+    const uint64_t v = (uint64_t) (uintptr_t) q;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t) v), hi = __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32));
+    return (const T*) (uintptr_t) (lo | ((uint64_t) hi << 32));
+}
+// 16 bytes of a weight, read once, at a scalar address and the lane's offset
+__device__ __forceinline__ u32x4 ldw16_at(const void* base, uint32_t off)
+{
+    return __builtin_nontemporal_load((const HMOE_GLOBAL u32x4*) ((const HMOE_GLOBAL char*) base + off));
+}
+
 // ---- the experts, gate and up to the weighted sum, in one launch ----
 // One workgroup a CU: 8 waves that stream weights, one that finishes what they sum and one that brings what they need next. The
 // work is a list of tickets, taken in order through one counter: first the gate/up tiles (8 TR gated values of one expert: slot
@@ -245,40 +269,47 @@ __device__ __forceinline__ int sum8(int v)
 // gate/up tiles are counted. So every wait ends, whatever else is on the card and however many of this launch's workgroups have
 // started (all the same it is bounded: past the bound the output is NaN).
 //
-// Weights are read 8 rows x 128 bytes a load, each wave its own slice of the depth, one item (12 loads of 1 KB or so a wave)
-// ahead, and multiplied by 4-wide integer dot products with the tokens' values out of LDS: an expert has one or two tokens of a
-// step, for which a matrix instruction would be mostly empty, and whole lines arrive faster from memory than a matrix
-// fragment's order (16 rows x 64 bytes): 7.0 against 5.7 TB/s over 3.2 GB. The streaming waves load nothing else: loads return
-// in order, so whatever they waited for would wait for the weights in flight.
+// Weights are read 8 rows x 128 bytes a load, each wave its own slice of the depth, and multiplied by 4-wide integer dot
+// products with the tokens' values out of LDS: an expert has one or two tokens of a step, for which a matrix instruction would
+// be mostly empty, and whole lines arrive faster from memory than a matrix fragment's order (16 rows x 64 bytes): 7.0 against
+// 5.7 TB/s over 3.2 GB. A wave holds one item's loads (8 to 14 KB) and asks for the next item's line as soon as it has used
+// one. Two items deep it is no faster (7.1 TB/s either way over 2.5 GB of expert tiles), and a round trip of the other two
+// waves, whose loads return in the order of the workgroup's, takes 6 us in place of 1.4: longer than an item. The streaming
+// waves load nothing else for the same reason, and the other two use what they ask for an item later.
 //
 // A wave's whole numbers are exact; those of a down tile are scaled and added slot by slot in fp32, then over the 8 waves: the
 // same order every time.
-constexpr int M8_ARENA = 140 * 1024, M8_RQ = 32;                        // LDS of x, partial sums and quantised rows; rows of a batch
+constexpr int M8_ARENA = 148 * 1024, M8_RQ = 32;                        // LDS of x, sums and quantised rows; rows of a batch
 
 template <int NS, int TR, int NSD>
 __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
 {
-    constexpr int NG2 = 2 * NS * TR, SB = NG2 / NSD < 6 ? (NG2 / NSD > 0 ? NG2 / NSD : 1) : 6;     // slots of a batch
-    constexpr int NL = NG2 > SB * NSD ? NG2 : SB * NSD;                 // loads of an item
-    constexpr int XP = 1024 * NS, ROWS = 16 * TR;                       // LDS row of x; rows of a gate/up tile
-    static_assert(M8_T * (XP + 64 * ROWS) <= M8_ARENA && 2 * M8_T * 1024 * NSD <= M8_ARENA, "LDS");
+    constexpr int NG2 = 2 * NS * TR, SU = NG2 / NSD < 6 ? (NG2 / NSD > 0 ? NG2 / NSD : 1) : 6;     // (slot, 8 rows) pairs of a down item
+    constexpr int NL = NG2;                                             // loads of an item
+    static_assert(SU * NSD <= NL, "a down item fits the registers of a gate/up one");
+    constexpr int XP = 1024 * NS, ROWS = 16 * TR, QP = 1024 * NSD;      // LDS row of x; rows of a gate/up tile; LDS row of a batch
+    constexpr int RDM = NSD == 4 ? 2 : SU < 3 ? SU : 3;                 // 8-row groups of a down tile, at most
+    static_assert(M8_T * (XP + 64 * ROWS) <= M8_ARENA && M8_T * (2 * QP + 512 * RDM) <= M8_ARENA, "LDS");
     __shared__ M8Plan s;
     __shared__ __attribute__((aligned(16))) int8_t arena[M8_ARENA];
-    __shared__ float accl[2][8][8][M8_T];
     __shared__ float fq[2][M8_RQ];
     __shared__ uint16_t bst[M8_SLOTS + 1];                              // first slot of each batch
-    __shared__ int tk[4], nbl;
+    __shared__ int tk[8], nbl, late;
     const int t = threadIdx.x, l = t & 63, r = l >> 3, pc = l & 7;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-    constexpr int QP = 1024 * NSD;                                      // LDS row of a batch
     const int T = p.T, IP = (int) up128(p.I), HP = (int) up128(p.H);
-    // x [T][XP], partial sums [2][8][ROWS][T] and the batches' rows [2][rq][QP]: side by side, or the rows in the others' place
+    // a down tile: as many 8-row groups as give each of 256 workgroups one, so that the slots quantised last come last in it
+    const int RD = min(cdiv(p.H, 8 * 256), RDM), SB = SU / RD;
+    // x [T][XP] and partial sums [2][8][ROWS][T]; a down tile's sums [2][8][8 RD][T] and the batches' rows [2][rq][QP]: side by
+    // side, or the later ones in the earlier ones' place
+    const int xr_bytes = T * (XP + 64 * ROWS), acc_bytes = 512 * RD * T;
+    const bool apart = xr_bytes + acc_bytes + 2 * T * QP <= M8_ARENA;
+    const int after = (apart ? xr_bytes : 0) + acc_bytes;
     int8_t* xl = arena;
     int* red = (int*) (arena + T * XP);
-    const int xr_bytes = T * (XP + 64 * ROWS);
-    const bool apart = xr_bytes + 2 * T * QP <= M8_ARENA;
-    int8_t* qb = apart ? arena + xr_bytes : arena;
-    const int rq = min((M8_ARENA - (apart ? xr_bytes : 0)) / (2 * QP), M8_RQ);
+    float* accl = (float*) (arena + after - acc_bytes);
+    int8_t* qb = arena + after;
+    const int rq = min((M8_ARENA - after) / (2 * QP), M8_RQ);
     if (t == 0)
     {
         const int v = __hip_atomic_fetch_add(p.ticket, 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -289,75 +320,162 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         const int tok = i / (XP / 16), k = 16 * (i - tok * (XP / 16));
         *(u32x4*) (xl + tok * XP + k) = k < p.H ? ld16(p.xq + (size_t) tok * HP + k) : (u32x4) {0u, 0u, 0u, 0u};
     }
+    const int NB = cdiv(p.I, 8 * TR);
+    // a streaming wave's slice of the depth is NS (gate, up) or NSD (down) lines of 128 bytes from line w NS (w NSD) on; a piece
+    // behind the depth re-reads the row's last 16 bytes, against values that are zero. Rows come in whole groups of 8 (H and I
+    // are multiples of 16), so that a load is a scalar address and one of these lane offsets
+    uint32_t vo[NS], vd[NSD];
+    #pragma unroll
+    for (int i = 0; i < NS; ++i) vo[i] = (uint32_t) (r * p.H + min(128 * (w * NS + i) + 16 * pc, p.H - 16));
+    #pragma unroll
+    for (int i = 0; i < NSD; ++i) vd[i] = (uint32_t) (r * p.I + min(128 * (w * NSD + i) + 16 * pc, p.I - 16));
+    u32x4 a[NL];
+    float sd[SU];
+    // (held in scalar registers: where the choice between an expert's and the shared expert's matrix became a choice between two
+    // kernel arguments to load, the load went the weights' way, behind all of them)
+    const int8_t *wg = p.wg, *wu = p.wu, *wd = p.wd, *hg = p.hg, *hu = p.hu, *hd = p.hd;
+    const float *wsd = p.sd, *hsd = p.hsd;
+    asm volatile("" : "+s"(wg), "+s"(wu), "+s"(wd), "+s"(hg), "+s"(hu), "+s"(hd), "+s"(wsd), "+s"(hsd));
+    struct GuAt { const int8_t* g[TR]; const int8_t* u[TR]; };
+    auto gu_at = [&](int expert, int blk) {                              // expert -1: the shared one
+        GuAt o;
+        const size_t eo = expert < 0 ? 0 : (size_t) expert * p.I * p.H;
+        #pragma unroll
+        for (int tr = 0; tr < TR; ++tr)
+        {
+            const size_t ro = eo + (size_t) min(TR * blk + tr, p.I / 8 - 1) * 8 * p.H;
+            o.g[tr] = scalar((expert < 0 ? hg : wg) + ro);
+            o.u[tr] = scalar((expert < 0 ? hu : wu) + ro);
+        }
+        return o;
+    };
+    auto load_gu = [&](const GuAt& at, int i, int tr) {                  // line i of group tr of both
+        a[tr * NS + i] = ldw16_at(at.g[tr], vo[i]);
+        a[(TR + tr) * NS + i] = ldw16_at(at.u[tr], vo[i]);
+    };
+    __syncthreads();
+    // the shared expert's first tiles need no plan: their weights come while it is made
+    const int first = __builtin_amdgcn_readfirstlane(tk[0]);
+    const bool early = p.hg && first < NB;
+    if (early && w < 8)
+    {
+        const GuAt at = gu_at(-1, first);
+        #pragma unroll
+        for (int i = 0; i < NS; ++i)
+            #pragma unroll
+            for (int tr = 0; tr < TR; ++tr) load_gu(at, i, tr);
+    }
     m8_plan(p, s, blockIdx.x == 0);
-    const int slots = s.slots, NB = cdiv(p.I, 8 * TR), NG = slots * NB, total = NG + cdiv(p.H, 8);
+    const int slots = __builtin_amdgcn_readfirstlane(s.slots), NG = slots * NB, total = NG + cdiv(p.H, 8 * RD);
     if (t == 0)
     {
-        int n = 0, first = 0;
+        int n = 0, from = 0;
         for (int sl = 0; sl < slots; ++sl)
-            if (sl == 0 || sl - first == SB || s.row0[sl + 1] - s.row0[first] > rq) { bst[n++] = (uint16_t) sl; first = sl; }
+            if (sl == 0 || sl - from == SB || s.row0[sl + 1] - s.row0[from] > rq) { bst[n++] = (uint16_t) sl; from = sl; }
         bst[n] = (uint16_t) slots;
         nbl = n;
     }
     __syncthreads();
-    const int nb = max(nbl, 1);                                         // batches of a down tile
+    const int nb = max(__builtin_amdgcn_readfirstlane(nbl), 1);                                         // batches of a down tile
 
     // an item: a gate/up tile (batch < 0) or one batch of a down tile; d counts the down items
     struct Item { int ticket, seq, slot, blk, batch, d; };
     auto item = [&](int ticket, int seq, int d) {
         Item it = {ticket, seq, 0, 0, -1, d};
-        if (ticket < NG) { it.slot = ticket / NB; it.blk = ticket - it.slot * NB; }
+        if (ticket < NG) { it.slot = (int) ((uint32_t) ticket / (uint32_t) NB); it.blk = ticket - it.slot * NB; }
         else { it.blk = ticket - NG; it.batch = 0; ++it.d; }
         return it;
     };
     auto next = [&](const Item& c) {
         if (c.batch >= 0 && c.batch + 1 < nb) { Item it = c; ++it.batch; ++it.d; return it; }
-        return item(__builtin_amdgcn_readfirstlane(tk[(c.seq + 1) & 3]), c.seq + 1, c.d);
+        return item(__builtin_amdgcn_readfirstlane(tk[(c.seq + 1) & 7]), c.seq + 1, c.d);
     };
-    // between the last gate/up tile and the first down batch: what is brought then may wait for this workgroup's own tiles
+    // between the last gate/up tile and the first down batch: what was not ready then is brought, and may wait for this
+    // workgroup's own tiles
     auto turns = [&](const Item& c, const Item& n) { return c.batch < 0 && n.batch >= 0 && n.ticket < total; };
-    Item cur = item(__builtin_amdgcn_readfirstlane(tk[0]), 0, 0);
+    auto turn = [&](const Item& c, const Item& n) {
+        if (!turns(c, n) || !__builtin_amdgcn_readfirstlane(late)) return;
+        if (!apart) __syncthreads();
+        __syncthreads();
+    };
+    Item cur = item(first, 0, 0);
 
     if (w == 9)
     {
         // the bringing wave: tickets, and the rows of the next down batch
-        int ready = 0;                                                   // slots below it are known to be quantised
+        int ready = 0, seen = 0;                                         // slots below ready are known to be quantised
         bool lost = false;
+        auto ask = [&]() {
+            const int f = ready + l;
+            return f < slots ? __hip_atomic_load(p.flag + f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        };
+        auto hear = [&](int v) {
+            const unsigned long long up = __ballot(v != 0);
+            ready += up == ~0ull ? 64 : __builtin_ctzll(~up);
+        };
         auto bring = [&](const Item& it) {
             if (it.batch < 0 || it.ticket >= total || slots == 0) return;
             const int s0 = bst[it.batch], s1 = bst[it.batch + 1], r0 = s.row0[s0], n = s.row0[s1] - r0;
             for (int polls = 0; ready < s1 && !lost; ++polls)
             {
-                const int f = ready + l;
-                const int v = f < slots ? __hip_atomic_load(p.flag + f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-                const unsigned long long up = __ballot(v != 0);
-                ready += up == ~0ull ? 64 : __builtin_ctzll(~up);
+                hear(ask());
                 if (ready < s1) __builtin_amdgcn_s_sleep(4);
                 lost = polls > (1 << 22);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-            int8_t* q = qb + (it.d & 1) * rq * QP;
-            #pragma unroll 8
-            for (int i = l; i < n * (QP / 16); i += 64)
+            if (seen < s1)
             {
-                const int row = i / (QP / 16), k = 16 * (i % (QP / 16));
-                *(u32x4*) (q + 16 * i) = k < p.I ? ld16(p.qa + (size_t) (r0 + row) * IP + k) : (u32x4) {0u, 0u, 0u, 0u};
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+                seen = ready;
             }
-            if (l < n) fq[it.d & 1][l] = lost ? __uint_as_float(0x7fc00000u) : p.sa[r0 + l] * s.weight[r0 + l];
+            int8_t* q = qb + (it.d & 1) * rq * QP;
+            const float f = l < n ? p.sa[r0 + l] : 0.f;
+            const int pieces = n * (QP / 16);
+            for (int i0 = 0; i0 < pieces; i0 += 512)
+            {
+                u32x4 v[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                {
+                    const int i = min(i0 + 64 * j + l, pieces - 1);
+                    v[j] = ld16(p.qa + (size_t) (r0 + i / (QP / 16)) * IP + min(16 * (i % (QP / 16)), p.I - 16));
+                }
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                {
+                    const int i = i0 + 64 * j + l;
+                    if (i < pieces) *(u32x4*) (q + 16 * i) = 16 * (i % (QP / 16)) < p.I ? v[j] : (u32x4) {0u, 0u, 0u, 0u};
+                }
+            }
+            if (l < n) fq[it.d & 1][l] = lost ? __uint_as_float(0x7fc00000u) : f * s.weight[r0 + l];
         };
         bring(cur);
+        int nt = 0;
+        if (l == 0) nt = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        int flags = 0;
         __syncthreads();
         while (cur.ticket < total)
         {
-            const bool fetch = cur.batch <= 0;                           // the ticket after the next: one a ticket
-            int nt = 0;
-            if (fetch && l == 0) nt = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            // a ticket a ticket, and a look at the flags: what the item before asked for
+            if (cur.batch <= 0)
+            {
+                if (l == 0)
+                {
+                    tk[(cur.seq + 2) & 7] = nt;
+                    nt = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                if (cur.batch < 0)
+                {
+                    hear(flags);
+                    flags = ask();
+                }
+            }
             const Item nx = next(cur);
-            const bool turn = turns(cur, nx);
-            if (!turn) bring(nx);
-            if (fetch && l == 0) tk[(cur.seq + 2) & 3] = nt;
+            const bool tn = turns(cur, nx);
+            const bool now = !tn || (apart && (slots == 0 || ready >= bst[1]));
+            if (now) bring(nx);
+            if (tn && l == 0) late = !now;
             __syncthreads();
-            if (turn)
+            if (!now)
             {
                 if (!apart) __syncthreads();
                 bring(nx);
@@ -369,27 +487,77 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     }
     if (w == 8)
     {
-        // the finishing wave; the next tile's scales are on their way while it finishes one
+        // the finishing wave. A tile's values are stored in its item, counted in the next (behind the wait for that one's scales,
+        // which were asked for after them), and the count is looked at in the one after
         float sg = 0.f, su = 0.f;
         auto scales = [&](const Item& it) {
-            if (it.batch >= 0 || l >= 8 * TR) return;
+            if (it.batch >= 0 || it.ticket >= total || l >= 8 * TR) return;
             const bool sh = p.hg && it.slot == 0;
             const size_t so = (sh ? 0 : (size_t) s.expert[it.slot] * p.I) + min(8 * TR * it.blk + l, p.I - 1);
             sg = (sh ? p.hsg : p.sg)[so];
             su = (sh ? p.hsu : p.su)[so];
         };
-        if (cur.ticket < total) scales(cur);
+        int stored = -1, counted = -1, done = 0;                         // slots of the tiles stored and counted last
+        auto count = [&]() {
+            if (stored >= 0 && l == 0) done = __hip_atomic_fetch_add(p.count + 32 * stored, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            counted = stored;
+            stored = -1;
+        };
+        // a slot whose tiles are all counted: its rows in 8 bits. The values come past this XCD's caches (as they were stored),
+        // and go the same way
+        auto look = [&]() {
+            if (counted < 0 || __builtin_amdgcn_readfirstlane(done) != NB - 1) { counted = -1; return; }
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            const int row0 = s.row0[counted], m = s.row0[counted + 1] - row0;
+            for (int k = 0; k < m; ++k)
+            {
+                constexpr int G = M8_I / 16 / 64;
+                const float* h = p.act + (size_t) (row0 + k) * p.I;
+                float v[G][16];
+                uint32_t top = 0;
+                #pragma unroll
+                for (int g = 0; g < G; ++g)
+                    if (1024 * g < p.I) load16<HMOE_DT_F32, true>(h, min(l + 64 * g, p.I / 16 - 1), v[g]);
+                #pragma unroll
+                for (int g = 0; g < G; ++g)
+                    if (1024 * g < p.I)
+                    {
+                        #pragma unroll
+                        for (int j = 0; j < 16; ++j) top = max(top, mag(v[g][j]));
+                    }
+                const RowQ q = row_q(wave_ext_u32<true>(top));
+                #pragma unroll
+                for (int g = 0; g < G; ++g)
+                    if (1024 * g < p.I && l + 64 * g < p.I / 16)
+                    {
+                        const u32x4 o = quant16<HMOE_DT_BF16>(v[g], q);
+                        unsigned long long* to = (unsigned long long*) (p.qa + (size_t) (row0 + k) * IP + 16 * (l + 64 * g));
+                        #pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            __hip_atomic_store(to + j, (unsigned long long) o[2 * j] | ((unsigned long long) o[2 * j + 1] << 32), __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT);
+                    }
+                if (l == 0) __hip_atomic_store(p.sa + row0 + k, q.s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (l == 0) __hip_atomic_store(p.flag + counted, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            counted = -1;
+        };
+        scales(cur);
         __syncthreads();
         while (cur.ticket < total)
         {
-            const bool gu = cur.batch < 0;
             const Item nx = next(cur);
             __syncthreads();
-            if (gu)
+            if (cur.batch < 0)
             {
                 const uint32_t mask = s.tokens[cur.slot];
                 const int m = __popc(mask), row0 = s.row0[cur.slot];
                 const int* rd = red + (cur.seq & 1) * 8 * ROWS * T;
+                // (values stored at the agent's scope go past the XCD's own L2: once the wait is over they can be seen, without
+                // writing the L2's lines back, which takes longer than a tile)
+                asm volatile("s_waitcnt vmcnt(0)" : "+v"(sg), "+v"(su) : : "memory");
+                look();
                 for (int i0 = 0; i0 < 8 * TR * m; i0 += 64)
                 {
                     const int i = min(i0 + l, 8 * TR * m - 1), k = i / (8 * TR), rr = i - k * 8 * TR, n = 8 * TR * cur.blk + rr;
@@ -407,182 +575,235 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
                     if (i0 + l < 8 * TR * m && n < p.I)
                         __hip_atomic_store(p.act + (size_t) (row0 + k) * p.I + n, swiglu(g, u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                if (nx.ticket < total) scales(nx);
-                // (the values were stored past the XCD's own L2, as stores at the agent's scope are: once they are counted off they
-                // can be seen, without writing the L2's lines back first, which takes longer than a tile)
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                int done = 0;
-                if (l == 0) done = __hip_atomic_fetch_add(p.count + cur.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (__builtin_amdgcn_readfirstlane(done) == NB - 1)
+                count();
+                stored = cur.slot;
+                scales(nx);
+                if (nx.batch >= 0 || nx.ticket >= total)
                 {
-                    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-                    for (int k = 0; k < m; ++k)
-                    {
-                        const float* a = p.act + (size_t) (row0 + k) * p.I;
-                        uint32_t top = 0;
-                        for (int i = l; i < p.I / 16; i += 64)
-                        {
-                            float v[16];
-                            load16<HMOE_DT_F32, true>(a, i, v);
-                            #pragma unroll
-                            for (int j = 0; j < 16; ++j) top = max(top, mag(v[j]));
-                        }
-                        const RowQ q = row_q(wave_ext_u32<true>(top));
-                        for (int i = l; i < p.I / 16; i += 64)
-                        {
-                            float v[16];
-                            load16<HMOE_DT_F32, true>(a, i, v);
-                            *(u32x4*) (p.qa + (size_t) (row0 + k) * IP + 16 * i) = quant16<HMOE_DT_BF16>(v, q);
-                        }
-                        if (l == 0) p.sa[row0 + k] = q.s;
-                    }
-                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
-                    if (l == 0) __hip_atomic_store(p.flag + cur.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    // the last of this workgroup's gate/up tiles
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    look();
+                    count();
+                    look();
                 }
             }
             else if (cur.batch + 1 == nb)
             {
-                for (int i = l; i < 8 * T; i += 64)
+                const float* ac = accl + (cur.seq & 1) * 64 * RD * T;
+                for (int i = l; i < 8 * RD * T; i += 64)
                 {
-                    const int rr = i & 7, tok = i >> 3;
+                    const int tok = i / (8 * RD), rr = i - tok * 8 * RD;
                     float v = 0.f;
                     #pragma unroll
-                    for (int k = 0; k < 8; ++k) v += accl[cur.seq & 1][k][rr][tok];
-                    if (8 * cur.blk + rr < p.H) store_out(p.y, (size_t) tok * p.ldy + 8 * cur.blk + rr, v, p.ydt);
+                    for (int k = 0; k < 8; ++k) v += ac[(k * 8 * RD + rr) * T + tok];
+                    if (8 * RD * cur.blk + rr < p.H) store_out(p.y, (size_t) tok * p.ldy + 8 * RD * cur.blk + rr, v, p.ydt);
                 }
             }
-            if (turns(cur, nx))
-            {
-                if (!apart) __syncthreads();
-                __syncthreads();
-            }
+            turn(cur, nx);
             cur = nx;
         }
         return;
     }
 
-    // a streaming wave: its slice of the depth is NS (gate, up) or NSD (down) lines of 128 bytes from line w NS (w NSD) on; a
-    // piece behind the depth re-reads the row's last 16 bytes, against values that are taken as zero
-    u32x4 a[2][NL];
-    float sd[2][SB];
-    auto load = [&](const Item& it, u32x4 (&d)[NL], float (&sc)[SB]) {
-        if (it.ticket >= total) return;
-        if (it.batch < 0)
+    // a streaming wave
+    auto expert_of = [&](int slot) { return p.hg && slot == 0 ? -1 : __builtin_amdgcn_readfirstlane((int) s.expert[slot]); };
+    struct DnAt { const int8_t* w[SU]; const float* s[SU]; int live; };
+    auto dn_at = [&](const Item& it) {
+        // (a pair behind the batch's last asks for one piece of x: every item has the same number of loads to wait for)
+        DnAt o;
+        o.live = 0;
+        int sl = 0, s1 = 0, og = 0;
+        if (slots > 0)
         {
-            const bool sh = p.hg && it.slot == 0;
-            const size_t eo = sh ? 0 : (size_t) s.expert[it.slot] * p.I * p.H;
-            const int8_t* wg = (sh ? p.hg : p.wg) + eo;
-            const int8_t* wu = (sh ? p.hu : p.wu) + eo;
+            sl = __builtin_amdgcn_readfirstlane((int) bst[it.batch]);
+            s1 = __builtin_amdgcn_readfirstlane((int) bst[it.batch + 1]);
+        }
+        #pragma unroll
+        for (int b = 0; b < SU; ++b)
+        {
+            const int8_t* wb = p.xq;
+            const float* sb = p.xs;
+            if (sl < s1)
+            {
+                const int e = expert_of(sl), n0 = 8 * min(RD * it.blk + og, p.H / 8 - 1);
+                wb = (e < 0 ? hd : wd + (size_t) e * p.H * p.I) + (size_t) n0 * p.I;
+                sb = (e < 0 ? hsd : wsd + (size_t) e * p.H) + n0;
+                o.live = b + 1;
+            }
+            o.w[b] = scalar(wb);
+            o.s[b] = scalar(sb);
+            if (++og == RD) { og = 0; ++sl; }
+        }
+        return o;
+    };
+    auto load_dn = [&](const DnAt& at, int j) {                          // load j of a down item
+        const int b = j / NSD, i = j % NSD;
+        const uint32_t is = b < at.live ? ~0u : 0u;
+        a[j] = ldw16_at(at.w[b], vd[i] & is);
+        if (i == NSD - 1) sd[b] = *(const HMOE_GLOBAL float*) ((const HMOE_GLOBAL char*) at.s[b] + (4u * r & is));
+    };
+    // two tokens of a gate/up item (or one, twice), the k-th on; KIND: the next item, whose loads take the place of what is used:
+    // gate/up 0, down 1, none 2. (One form for one token and for two: what is loaded on two ways that meet is moved where they
+    // do, and waited for)
+    auto tokens = [&](const Item& it, int t0, int t1, int k0, int k1, auto kind, const GuAt& ng, const DnAt& nd) {
+        constexpr int KIND = decltype(kind)::value;
+        int* rd = red + ((it.seq & 1) * 8 + w) * ROWS * T;
+        const int8_t* x[2] = {xl + t0 * XP + 128 * w * NS + 16 * pc, xl + t1 * XP + 128 * w * NS + 16 * pc};
+        int g[2][TR], u[2][TR];
+        #pragma unroll
+        for (int n = 0; n < 2; ++n)
+            #pragma unroll
+            for (int tr = 0; tr < TR; ++tr) g[n][tr] = u[n][tr] = 0;
+        #pragma unroll
+        for (int i = 0; i < NS; ++i)
+        {
+            u32x4 xv[2];
+            #pragma unroll
+            for (int n = 0; n < 2; ++n) xv[n] = *(const u32x4*) (x[n] + 128 * i);
             #pragma unroll
             for (int tr = 0; tr < TR; ++tr)
             {
-                const size_t ro = (size_t) min(8 * (TR * it.blk + tr) + r, p.I - 1) * p.H;
                 #pragma unroll
-                for (int i = 0; i < NS; ++i)
+                for (int n = 0; n < 2; ++n)
                 {
-                    const int off = min(128 * (w * NS + i) + 16 * pc, p.H - 16);
-                    d[tr * NS + i] = ldw16(wg + ro + off);
-                    d[(TR + tr) * NS + i] = ldw16(wu + ro + off);
+                    g[n][tr] = dot16(a[tr * NS + i], xv[n], g[n][tr]);
+                    u[n][tr] = dot16(a[(TR + tr) * NS + i], xv[n], u[n][tr]);
                 }
-            }
-        }
-        else if (slots > 0)
-        {
-            const int n = min(8 * it.blk + r, p.H - 1), s0 = bst[it.batch], s1 = bst[it.batch + 1];
-            #pragma unroll
-            for (int b = 0; b < SB; ++b)
-            {
-                const int sl = s0 + b;
-                if (sl >= s1) break;
-                const bool sh = p.hg && sl == 0;
-                const int8_t* wd = (sh ? p.hd : p.wd + (size_t) s.expert[sl] * p.H * p.I) + (size_t) n * p.I;
-                #pragma unroll
-                for (int i = 0; i < NSD; ++i) d[b * NSD + i] = ldw16(wd + min(128 * (w * NSD + i) + 16 * pc, p.I - 16));
-                sc[b] = (sh ? p.hsd : p.sd + (size_t) s.expert[sl] * p.H)[n];
-            }
-        }
-    };
-    auto compute = [&](const Item& it, const u32x4 (&d)[NL], const float (&sc)[SB]) {
-        if (it.batch < 0)
-        {
-            int* rd = red + ((it.seq & 1) * 8 + w) * ROWS * T;
-            int k = 0;
-            for (uint32_t m = s.tokens[it.slot]; m; m &= m - 1, ++k)
-            {
-                const int8_t* x = xl + __builtin_ctz(m) * XP + 128 * w * NS + 16 * pc;
-                int g[TR], u[TR];
-                #pragma unroll
-                for (int tr = 0; tr < TR; ++tr) g[tr] = u[tr] = 0;
-                #pragma unroll
-                for (int i = 0; i < NS; ++i)
+                if constexpr (KIND < 2)
                 {
-                    const u32x4 xv = *(const u32x4*) (x + 128 * i);
+                    // (the products stand here: where they are put off, the loads below get other registers, and the moves back wait
+                    // for them)
                     #pragma unroll
-                    for (int tr = 0; tr < TR; ++tr)
+                    for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(g[n][tr]), "+v"(u[n][tr]));
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (KIND == 0) load_gu(ng, i, tr);
+                    else
                     {
-                        g[tr] = dot16(d[tr * NS + i], xv, g[tr]);
-                        u[tr] = dot16(d[(TR + tr) * NS + i], xv, u[tr]);
+                        if (tr * NS + i < SU * NSD) load_dn(nd, tr * NS + i);
+                        if ((TR + tr) * NS + i < SU * NSD) load_dn(nd, (TR + tr) * NS + i);
                     }
-                }
-                #pragma unroll
-                for (int tr = 0; tr < TR; ++tr)
-                {
-                    const int gs = sum8(g[tr]), us = sum8(u[tr]);
-                    if (pc == 0)
-                    {
-                        rd[(8 * tr + r) * T + k] = gs;
-                        rd[(8 * (TR + tr) + r) * T + k] = us;
-                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            return;
         }
-        float (*acc)[M8_T] = accl[it.seq & 1][w];
+        const int kk[2] = {k0, k1};
+        #pragma unroll
+        for (int n = 0; n < 2; ++n)
+            #pragma unroll
+            for (int tr = 0; tr < TR; ++tr)
+            {
+                const int gs = sum8(g[n][tr]), us = sum8(u[n][tr]);
+                if (pc == 0)
+                {
+                    rd[(8 * tr + r) * T + kk[n]] = gs;
+                    rd[(8 * (TR + tr) + r) * T + kk[n]] = us;
+                }
+            }
+    };
+    auto gate_up = [&](const Item& it, auto kind, const GuAt& ng, const DnAt& nd) {
+        uint32_t m = __builtin_amdgcn_readfirstlane((int) s.tokens[it.slot]);
+        int k = 0;
+        for (; __popc(m) > 2; k += 2)
+        {
+            const uint32_t m1 = m & (m - 1);
+            tokens(it, __builtin_ctz(m), __builtin_ctz(m1), k, k + 1, ic<2>{}, ng, nd);
+            m = m1 & (m1 - 1);
+        }
+        const uint32_t m1 = m & (m - 1);
+        tokens(it, __builtin_ctz(m), __builtin_ctz(m1 ? m1 : m), k, k + (m1 ? 1 : 0), kind, ng, nd);
+    };
+    auto down = [&](const Item& it, auto kind, const DnAt& nd) {
+        constexpr int KIND = decltype(kind)::value;
+        float* acc = accl + ((it.seq & 1) * 8 + w) * 8 * RD * T;
         if (it.batch == 0)
-            for (int i = l; i < 8 * M8_T; i += 64) (&acc[0][0])[i] = 0.f;
-        if (slots == 0) return;
-        const int s0 = bst[it.batch], s1 = bst[it.batch + 1], r0 = s.row0[s0];
+            for (int i = l; i < 8 * RD * T; i += 64) acc[i] = 0.f;
+        int sl = 0, s1 = 0, r0 = 0, og = 0;
+        if (slots > 0)
+        {
+            sl = __builtin_amdgcn_readfirstlane((int) bst[it.batch]);
+            s1 = __builtin_amdgcn_readfirstlane((int) bst[it.batch + 1]);
+            r0 = s.row0[sl];
+        }
         const int8_t* qr = qb + (it.d & 1) * rq * QP + 128 * w * NSD + 16 * pc;
         const float* f = fq[it.d & 1];
         #pragma unroll
-        for (int b = 0; b < SB; ++b)
+        for (int b = 0; b < SU; ++b)
         {
-            const int sl = s0 + b;
-            if (sl >= s1) break;
-            int row = s.row0[sl] - r0;
-            for (uint32_t m = s.tokens[sl]; m; m &= m - 1, ++row)
+            if (sl < s1)
             {
-                int v = 0;
+                int row = s.row0[sl] - r0;
+                for (uint32_t m = __builtin_amdgcn_readfirstlane((int) s.tokens[sl]); m; m &= m - 1, ++row)
+                {
+                    int v = 0;
+                    #pragma unroll
+                    for (int i = 0; i < NSD; ++i) v = dot16(a[b * NSD + i], *(const u32x4*) (qr + row * QP + 128 * i), v);
+                    v = sum8(v);
+                    if (pc == 0) acc[(8 * og + r) * T + __builtin_ctz(m)] += (float) v * (f[row] * sd[b]);
+                }
+            }
+            if (++og == RD) { og = 0; ++sl; }
+            if constexpr (KIND == 1)
+            {
+                __builtin_amdgcn_sched_barrier(0);
                 #pragma unroll
-                for (int i = 0; i < NSD; ++i) v = dot16(d[b * NSD + i], *(const u32x4*) (qr + row * QP + 128 * i), v);
-                v = sum8(v);
-                if (pc == 0) acc[r][__builtin_ctz(m)] += (float) v * (f[row] * sc[b]);
+                for (int i = 0; i < NSD; ++i) load_dn(nd, b * NSD + i);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
-    auto turn = [&](const Item& c, const Item& n) {
-        if (!turns(c, n)) return;
-        if (!apart) __syncthreads();
-        __syncthreads();
-    };
-    load(cur, a[0], sd[0]);
-    __syncthreads();
-    while (cur.ticket < total)
+    GuAt ng;
+    DnAt nd;
+    if (!early && cur.ticket < total)
     {
-        Item nx = next(cur);
-        load(nx, a[1], sd[1]);
-        compute(cur, a[0], sd[0]);
-        __syncthreads();
-        turn(cur, nx);
-        cur = nx;
-        if (cur.ticket >= total) break;
-        nx = next(cur);
-        load(nx, a[0], sd[0]);
-        compute(cur, a[1], sd[1]);
-        __syncthreads();
-        turn(cur, nx);
-        cur = nx;
+        if (cur.batch < 0)
+        {
+            ng = gu_at(expert_of(cur.slot), cur.blk);
+            #pragma unroll
+            for (int i = 0; i < NS; ++i)
+                #pragma unroll
+                for (int tr = 0; tr < TR; ++tr) load_gu(ng, i, tr);
+        }
+        else
+        {
+            nd = dn_at(cur);
+            #pragma unroll
+            for (int j = 0; j < SU * NSD; ++j) load_dn(nd, j);
+        }
     }
+    __syncthreads();
+    Item nx = cur.ticket < total ? next(cur) : cur;
+    if (cur.ticket < total && cur.batch < 0)
+    {
+        while (nx.batch < 0)                                             // (every ticket behind the gate/up ones is a down one)
+        {
+            ng = gu_at(expert_of(nx.slot), nx.blk);
+            gate_up(cur, ic<0>{}, ng, nd);
+            __syncthreads();
+            cur = nx;
+            nx = next(cur);
+        }
+        if (nx.ticket < total)
+        {
+            nd = dn_at(nx);
+            gate_up(cur, ic<1>{}, ng, nd);
+        }
+        else gate_up(cur, ic<2>{}, ng, nd);
+        __syncthreads();
+        turn(cur, nx);
+        cur = nx;
+        if (cur.ticket < total) nx = next(cur);
+    }
+    if (cur.ticket >= total) return;
+    while (nx.ticket < total)
+    {
+        nd = dn_at(nx);
+        down(cur, ic<1>{}, nd);
+        __syncthreads();
+        cur = nx;
+        nx = next(cur);
+    }
+    down(cur, ic<2>{}, nd);
+    __syncthreads();
 }
 
 template <int NS, int TR>
@@ -598,7 +819,7 @@ static size_t m8_layout(int T, int H, int I, int E, int topk, size_t* o)
 {
     const size_t rows = (size_t) T * (topk + 1);
     const size_t part[] = {(size_t) T * E * 8, (size_t) T * up128(H), (size_t) T * 4, rows * I * 4, rows * up128(I), rows * 4,
-                           (1 + 2 * M8_SLOTS) * 4};
+                           M8_SYNC * 4};
     size_t at = 0;
     for (int i = 0; i < 7; ++i)
     {
@@ -655,7 +876,7 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
                 sh_s ? sh_s[0] : nullptr, sh_s ? sh_s[1] : nullptr, sh_s ? sh_s[2] : nullptr,
                 T, H, I, E, n, lo, topk, scale, sel, rw, y, ldy, y_dtype,
                 (double*) (b + o[0]), (int8_t*) (b + o[1]), (float*) (b + o[2]), (float*) (b + o[3]), (int8_t*) (b + o[4]),
-                (float*) (b + o[5]), (int*) (b + o[6]), (int*) (b + o[6]) + 1, (int*) (b + o[6]) + 1 + M8_SLOTS};
+                (float*) (b + o[5]), (int*) (b + o[6]), (int*) (b + o[6]) + 32, (int*) (b + o[6]) + 32 + 32 * M8_SLOTS};
     const hipStream_t st = (hipStream_t) stream;
     const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * (x_dtype == HMOE_DT_F32 ? 4 : 2)) % 16 == 0;
 #define HMOE_R(D, V) m8_route_kernel<D, V><<<E + T, 256, 0, st>>>(p)
