@@ -8,7 +8,8 @@ namespace hmoe {
 constexpr int M8_T = 16, M8_K = 16, M8_E = 512, M8_H = 7168, M8_I = 4096;      // tokens, picks, experts, hidden and intermediate size
 constexpr int M8_SLOTS = M8_T * M8_K + 1;                             // distinct experts of a call, the shared one first
 constexpr int M8_ROWS = M8_T * (M8_K + 1);                            // (expert, token) rows of a call
-constexpr int M8_SYNC = 32 + 33 * M8_SLOTS;                           // the ticket counter, the slots' counts (a line each) and flags
+constexpr int M8_SUB = 8, M8_COPY = 32;                               // parts of a slot's count, copies of the rows' scales
+constexpr int M8_SYNC = 32 + 32 * M8_SUB * M8_SLOTS + M8_COPY * M8_ROWS;         // the claim counter, the slots' counts (a line each), the scales
 
 struct M8Args
 {
@@ -16,6 +17,7 @@ struct M8Args
     const float* wr; const float* bias;
     const int8_t* wg; const int8_t* wu; const int8_t* wd; const float* sg; const float* su; const float* sd;
     const int8_t* hg; const int8_t* hu; const int8_t* hd; const float* hsg; const float* hsu; const float* hsd;   // shared, or null
+    int64_t dg, du, dd, dsd;        // the shared expert's hg - wg, hu - wu, hd - wd, hsd - sd, in bytes
     int T, H, I, E, n, lo, topk;
     double scale;
     int64_t* sel; float* rw; void* y; int64_t ldy; int ydt;
@@ -23,8 +25,9 @@ struct M8Args
     double* logits;                 // [T][E]
     int8_t* xq; float* xs;          // [T][up128(H)], [T]
     float* act;                     // [rows][I]: silu(gate) up
-    int8_t* qa; float* sa;          // [rows][up128(I)], [rows]
-    int* ticket; int* count; int* flag;       // the next ticket; of each slot: gate/up tiles done, rows quantised
+    int8_t* qa;                     // [rows][up128(I)]
+    int* ticket; int* count;        // the next claim; of each slot, gate/up tiles done, in M8_SUB parts, a line each
+    uint32_t* up;                   // [M8_COPY][M8_ROWS]: a quantised row's scale with the sign set, 0 before
 };
 
 // ---- scores: one workgroup an expert, sums in 64 bits (scores next to each other decide the selection); behind them one
@@ -39,8 +42,7 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
     if ((int) blockIdx.x >= p.E)
     {
         const int row = blockIdx.x - p.E;
-        if (row == 0)
-            for (int i = t; i < M8_SYNC; i += 256) p.ticket[i] = 0;                // (ticket, count, flag: one array)
+        for (int i = row * 256 + t; i < M8_SYNC; i += p.T * 256) p.ticket[i] = 0;      // (ticket, count, up: one array)
         const uint8_t* xr = x + (size_t) row * p.ldx * es;
         uint32_t m = 0;
         for (int i = t; i < p.H / 16; i += 256)
@@ -117,9 +119,9 @@ __device__ inline unsigned long long order_key(double v)
 
 // The topk largest score + bias of token r by one wave: expert e is with lane e % 64, and each round takes the largest key left
 // and of equal ones the lowest id
+template <int EL>
 __device__ inline void m8_select(const M8Args& p, M8Plan& s, int r)
 {
-    constexpr int EL = M8_E / 64;
     const int l = threadIdx.x & 63;
     double a[EL];
     float bs[EL];
@@ -137,35 +139,39 @@ __device__ inline void m8_select(const M8Args& p, M8Plan& s, int r)
     #pragma unroll
     for (int i = 0; i < EL; ++i)
     {
-        k[i] = 0ull;
-        if (64 * i >= p.E) continue;
         a[i] = 1.0 / (1.0 + exp(-a[i]));
-        const int e = 64 * i + l;
-        if (e < p.E) k[i] = order_key(p.bias ? a[i] + (double) bs[i] : a[i]);
+        const unsigned long long o = order_key(p.bias ? a[i] + (double) bs[i] : a[i]);
+        k[i] = 64 * i + l < p.E ? o + 1ull : 0ull;                       // (the largest key is infinity's: + 1 does not wrap)
     }
-    uint32_t gone = 0;                                                   // the lane's experts that are taken
     for (int j = 0; j < p.topk; ++j)
     {
-        unsigned long long bk = 0ull;
-        int be = 0x7fffffff;
-        double ba = 0.0;
+        // the lane's best (of equal keys the lowest id, 0: none left), then the wave's: by the keys' upper halves, where those tie
+        // by the lower ones, and then by the ids
+        unsigned long long bk = k[0];
+        double ba = a[0];
+        int bi = 0;
         #pragma unroll
-        for (int i = 0; i < EL; ++i)
+        for (int i = 1; i < EL; ++i)
         {
-            const int e = 64 * i + l;
-            if (e >= p.E || ((gone >> i) & 1u) || (be != 0x7fffffff && k[i] <= bk)) continue;
-            bk = k[i]; be = e; ba = a[i];
+            const bool gt = k[i] > bk;
+            bk = gt ? k[i] : bk; ba = gt ? a[i] : ba; bi = gt ? i : bi;
         }
         const uint32_t hi = wave_ext_u32<true>((uint32_t) (bk >> 32));
-        const bool ch = (uint32_t) (bk >> 32) == hi && be != 0x7fffffff;
-        const uint32_t lo = wave_ext_u32<true>(ch ? (uint32_t) bk : 0u);
-        const bool cl = ch && (uint32_t) bk == lo;
-        const int e = (int) wave_ext_u32<false>(cl ? (uint32_t) be : 0x7fffffffu);
-        if (be == e)
+        bool c = (uint32_t) (bk >> 32) == hi;
+        unsigned long long who = __ballot(c);
+        if (who & (who - 1))
         {
-            gone |= 1u << (e >> 6);
-            s.sel[r][j] = e;
+            const uint32_t lo = wave_ext_u32<true>(c ? (uint32_t) bk : 0u);
+            c = c && (uint32_t) bk == lo;
+            const int e = (int) wave_ext_u32<false>(c ? (uint32_t) (64 * bi + l) : 0x7fffffffu);
+            who = 1ull << (e & 63);
+        }
+        if (l == __builtin_ctzll(who))
+        {
+            s.sel[r][j] = 64 * bi + l;
             s.top[r][j] = ba;
+            #pragma unroll
+            for (int i = 0; i < EL; ++i) k[i] = i == bi ? 0ull : k[i];
         }
     }
 }
@@ -176,7 +182,11 @@ __device__ inline void m8_plan(const M8Args& p, M8Plan& s, bool write)
     for (int e = t; e < M8_E; e += blockDim.x) s.mask[e] = 0;
     const int lt = t - (int) blockDim.x + 64;
     if (lt >= 0 && lt < p.T) s.xs[lt] = p.xs[lt];                        // (the last wave too)
-    for (int r = nw - 1 - (t >> 6); r < p.T; r += nw) m8_select(p, s, r);         // (the last waves first: they stream nothing)
+    for (int r = nw - 1 - (t >> 6); r < p.T; r += nw)                    // (the last waves first: they stream nothing)
+    {
+        if (p.E <= 256) m8_select<4>(p, s, r);
+        else m8_select<8>(p, s, r);
+    }
     __syncthreads();
     for (int i = t; i < p.T * p.topk; i += blockDim.x)
     {
@@ -264,9 +274,9 @@ __device__ __forceinline__ u32x4 ldw16_at(const void* base, uint32_t off)
 // work is a list of tickets, taken in order through one counter: first the gate/up tiles (8 TR gated values of one expert: slot
 // after slot, the shared expert first), then the down tiles (8 output columns, over every slot, a batch of slots at a time).
 //
-// A slot's last gate/up tile (by a count) quantises its rows and raises its flag; a down batch waits for its slots' flags. Those
-// come from earlier tickets alone, which are held by workgroups that run already; a workgroup waits for no flag before all its
-// gate/up tiles are counted. So every wait ends, whatever else is on the card and however many of this launch's workgroups have
+// Once a slot's gate/up tiles are counted, one workgroup quantises its rows and shows their scales; a down batch waits for its
+// rows' scales. Those come from earlier claims alone, which are held by workgroups that run already; a workgroup waits for none
+// before all its gate/up tiles are counted, and quantises what is left to it while it waits. So every wait ends, whatever else is on the card and however many of this launch's workgroups have
 // started (all the same it is bounded: past the bound the output is NaN).
 //
 // Weights are read 8 rows x 128 bytes a load, each wave its own slice of the depth, and multiplied by 4-wide integer dot
@@ -293,16 +303,14 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     __shared__ M8Plan s;
     __shared__ __attribute__((aligned(16))) int8_t arena[M8_ARENA];
     __shared__ float fq[2][M8_RQ];
-    __shared__ uint16_t bst[M8_SLOTS + 1];                              // first slot of each batch
-    __shared__ int tk[8], nbl, late;
+    __shared__ uint16_t duty[M8_SLOTS];                                 // the slots this workgroup is to quantise
+    __shared__ int tk[8], late;
     const int t = threadIdx.x, l = t & 63, r = l >> 3, pc = l & 7;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int T = p.T, IP = (int) up128(p.I), HP = (int) up128(p.H);
-    // a down tile: as many 8-row groups as give each of 256 workgroups one, so that the slots quantised last come last in it
-    const int RD = min(cdiv(p.H, 8 * 256), RDM), SB = SU / RD;
     // x [T][XP] and partial sums [2][8][ROWS][T]; a down tile's sums [2][8][8 RD][T] and the batches' rows [2][rq][QP]: side by
     // side, or the later ones in the earlier ones' place
-    const int xr_bytes = T * (XP + 64 * ROWS), acc_bytes = 512 * RD * T;
+    const int xr_bytes = T * (XP + 64 * ROWS), acc_bytes = 512 * min(cdiv(p.H, 8 * 256), RDM) * T;
     const bool apart = xr_bytes + acc_bytes + 2 * T * QP <= M8_ARENA;
     const int after = (apart ? xr_bytes : 0) + acc_bytes;
     int8_t* xl = arena;
@@ -310,11 +318,8 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     float* accl = (float*) (arena + after - acc_bytes);
     int8_t* qb = arena + after;
     const int rq = min((M8_ARENA - after) / (2 * QP), M8_RQ);
-    if (t == 0)
-    {
-        const int v = __hip_atomic_fetch_add(p.ticket, 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        tk[0] = v; tk[1] = v + 1;
-    }
+    auto claim = [&]() { return __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    if (t == 0) tk[0] = claim();
     for (int i = t; i < T * (XP / 16); i += 640)
     {
         const int tok = i / (XP / 16), k = 16 * (i - tok * (XP / 16));
@@ -331,21 +336,19 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     for (int i = 0; i < NSD; ++i) vd[i] = (uint32_t) (r * p.I + min(128 * (w * NSD + i) + 16 * pc, p.I - 16));
     u32x4 a[NL];
     float sd[SU];
-    // (held in scalar registers: where the choice between an expert's and the shared expert's matrix became a choice between two
-    // kernel arguments to load, the load went the weights' way, behind all of them)
-    const int8_t *wg = p.wg, *wu = p.wu, *wd = p.wd, *hg = p.hg, *hu = p.hu, *hd = p.hd;
-    const float *wsd = p.sd, *hsd = p.hsd;
-    asm volatile("" : "+s"(wg), "+s"(wu), "+s"(wd), "+s"(hg), "+s"(hu), "+s"(hd), "+s"(wsd), "+s"(hsd));
+    // (the shared expert's matrices as distances from the others: a choice between two kernel arguments became a choice of which to
+    // load, and that load went the weights' way, behind all of them)
     struct GuAt { const int8_t* g[TR]; const int8_t* u[TR]; };
     auto gu_at = [&](int expert, int blk) {                              // expert -1: the shared one
         GuAt o;
-        const size_t eo = expert < 0 ? 0 : (size_t) expert * p.I * p.H;
+        const int64_t eo = (int64_t) expert * p.I * p.H;
+        const uintptr_t g = (uintptr_t) p.wg + (expert < 0 ? p.dg : eo), u = (uintptr_t) p.wu + (expert < 0 ? p.du : eo);
         #pragma unroll
         for (int tr = 0; tr < TR; ++tr)
         {
-            const size_t ro = eo + (size_t) min(TR * blk + tr, p.I / 8 - 1) * 8 * p.H;
-            o.g[tr] = scalar((expert < 0 ? hg : wg) + ro);
-            o.u[tr] = scalar((expert < 0 ? hu : wu) + ro);
+            const size_t ro = (size_t) min(TR * blk + tr, p.I / 8 - 1) * 8 * p.H;
+            o.g[tr] = scalar((const int8_t*) (g + ro));
+            o.u[tr] = scalar((const int8_t*) (u + ro));
         }
         return o;
     };
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     __syncthreads();
     // the shared expert's first tiles need no plan: their weights come while it is made
     const int first = __builtin_amdgcn_readfirstlane(tk[0]);
-    const bool early = p.hg && first < NB;
+    const bool early = p.hg && T <= 2 && first < min(NB, 256);           // (more tokens are selected by the streaming waves too)
     if (early && w < 8)
     {
         const GuAt at = gu_at(-1, first);
@@ -366,17 +369,15 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
             for (int tr = 0; tr < TR; ++tr) load_gu(at, i, tr);
     }
     m8_plan(p, s, blockIdx.x == 0);
-    const int slots = __builtin_amdgcn_readfirstlane(s.slots), NG = slots * NB, total = NG + cdiv(p.H, 8 * RD);
-    if (t == 0)
-    {
-        int n = 0, from = 0;
-        for (int sl = 0; sl < slots; ++sl)
-            if (sl == 0 || sl - from == SB || s.row0[sl + 1] - s.row0[from] > rq) { bst[n++] = (uint16_t) sl; from = sl; }
-        bst[n] = (uint16_t) slots;
-        nbl = n;
-    }
-    __syncthreads();
-    const int nb = max(__builtin_amdgcn_readfirstlane(nbl), 1);                                         // batches of a down tile
+    const int slots = __builtin_amdgcn_readfirstlane(s.slots);
+    // a down tile: as many 8-row groups as give each of 256 workgroups one, so that the slots quantised last come last in it
+    const int RD = min(cdiv(p.H, 8 * 256), RDM), SB = max(min(SU / RD, rq / T), 1);
+    const int NG = slots * NB, total = NG + cdiv(p.H, 8 * RD);
+    // claims, one atomic each: the first 256 stand for `run` gate/up tiles, 256 apart (so that all work on the same slot), the
+    // others for one ticket. (A claim for each tile from every workgroup kept one line of memory busy for longer than the tile)
+    const int run = max(NG / 256 - 1, 1);
+    auto ticket_of = [&](int c) { return c < 256 ? c : 256 * (run - 1) + c; };
+    const int nb = max(cdiv(slots, SB), 1);                             // batches of a down tile
 
     // an item: a gate/up tile (batch < 0) or one batch of a down tile; d counts the down items
     struct Item { int ticket, seq, slot, blk, batch, d; };
@@ -398,126 +399,46 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         if (!apart) __syncthreads();
         __syncthreads();
     };
-    Item cur = item(first, 0, 0);
+    const int start = ticket_of(first);
+    Item cur = item(start, 0, 0);
 
     if (w == 9)
     {
         // the bringing wave: tickets, and the rows of the next down batch
-        int ready = 0, seen = 0;                                         // slots below ready are known to be quantised
+        // (each workgroup looks at one of 32 copies of the rows' scales: a line that all of them read past their caches is served to
+        // one after the other)
+        const uint32_t* up = p.up + (blockIdx.x % M8_COPY) * M8_ROWS;
         bool lost = false;
-        auto ask = [&]() {
-            const int f = ready + l;
-            return f < slots ? __hip_atomic_load(p.flag + f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        auto ask = [&](const Item& it, uint32_t& v) __attribute__((always_inline)) {                    // whether the batch's rows are there; their scales
+            const int r0 = s.row0[it.batch * SB], n = s.row0[min((it.batch + 1) * SB, slots)] - r0;
+            v = l < n ? __hip_atomic_load(up + r0 + l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 1u;
+            return __ballot(v == 0u) == 0ull;
         };
-        auto hear = [&](int v) {
-            const unsigned long long up = __ballot(v != 0);
-            ready += up == ~0ull ? 64 : __builtin_ctzll(~up);
-        };
-        auto bring = [&](const Item& it) {
-            if (it.batch < 0 || it.ticket >= total || slots == 0) return;
-            const int s0 = bst[it.batch], s1 = bst[it.batch + 1], r0 = s.row0[s0], n = s.row0[s1] - r0;
-            for (int polls = 0; ready < s1 && !lost; ++polls)
-            {
-                hear(ask());
-                if (ready < s1) __builtin_amdgcn_s_sleep(4);
-                lost = polls > (1 << 22);
-            }
-            if (seen < s1)
-            {
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-                seen = ready;
-            }
-            int8_t* q = qb + (it.d & 1) * rq * QP;
-            const float f = l < n ? p.sa[r0 + l] : 0.f;
-            const int pieces = n * (QP / 16);
-            for (int i0 = 0; i0 < pieces; i0 += 512)
-            {
-                u32x4 v[8];
-                #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                {
-                    const int i = min(i0 + 64 * j + l, pieces - 1);
-                    v[j] = ld16(p.qa + (size_t) (r0 + i / (QP / 16)) * IP + min(16 * (i % (QP / 16)), p.I - 16));
-                }
-                #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                {
-                    const int i = i0 + 64 * j + l;
-                    if (i < pieces) *(u32x4*) (q + 16 * i) = 16 * (i % (QP / 16)) < p.I ? v[j] : (u32x4) {0u, 0u, 0u, 0u};
-                }
-            }
-            if (l < n) fq[it.d & 1][l] = lost ? __uint_as_float(0x7fc00000u) : f * s.weight[r0 + l];
-        };
-        bring(cur);
-        int nt = 0;
-        if (l == 0) nt = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        int flags = 0;
-        __syncthreads();
-        while (cur.ticket < total)
-        {
-            // a ticket a ticket, and a look at the flags: what the item before asked for
-            if (cur.batch <= 0)
-            {
-                if (l == 0)
-                {
-                    tk[(cur.seq + 2) & 7] = nt;
-                    nt = __hip_atomic_fetch_add(p.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
-                if (cur.batch < 0)
-                {
-                    hear(flags);
-                    flags = ask();
-                }
-            }
-            const Item nx = next(cur);
-            const bool tn = turns(cur, nx);
-            const bool now = !tn || (apart && (slots == 0 || ready >= bst[1]));
-            if (now) bring(nx);
-            if (tn && l == 0) late = !now;
-            __syncthreads();
-            if (!now)
-            {
-                if (!apart) __syncthreads();
-                bring(nx);
-                __syncthreads();
-            }
-            cur = nx;
-        }
-        return;
-    }
-    if (w == 8)
-    {
-        // the finishing wave. A tile's values are stored in its item, counted in the next (behind the wait for that one's scales,
-        // which were asked for after them), and the count is looked at in the one after
-        float sg = 0.f, su = 0.f;
-        auto scales = [&](const Item& it) {
-            if (it.batch >= 0 || it.ticket >= total || l >= 8 * TR) return;
-            const bool sh = p.hg && it.slot == 0;
-            const size_t so = (sh ? 0 : (size_t) s.expert[it.slot] * p.I) + min(8 * TR * it.blk + l, p.I - 1);
-            sg = (sh ? p.hsg : p.sg)[so];
-            su = (sh ? p.hsu : p.su)[so];
-        };
-        int stored = -1, counted = -1, done = 0;                         // slots of the tiles stored and counted last
-        auto count = [&]() {
-            if (stored >= 0 && l == 0) done = __hip_atomic_fetch_add(p.count + 32 * stored, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            counted = stored;
-            stored = -1;
-        };
-        // a slot whose tiles are all counted: its rows in 8 bits. The values come past this XCD's caches (as they were stored),
-        // and go the same way
-        auto look = [&]() {
-            if (counted < 0 || __builtin_amdgcn_readfirstlane(done) != NB - 1) { counted = -1; return; }
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-            const int row0 = s.row0[counted], m = s.row0[counted + 1] - row0;
+        // The workgroup that took one certain tile of a slot, another one for each slot, brings the slot's rows into 8 bits once all
+        // its tiles are counted. (Left to whoever counts the last tile, the slowest workgroup gets every slot, and is slower for
+        // it.) The values come past this XCD's caches, as they were stored, and go the same way
+        int head = 0, tail = 0;
+        auto quantise = [&](int slot) __attribute__((always_inline)) {
+            constexpr int G = M8_I / 16 / 64;
+            const int row0 = s.row0[slot], m = s.row0[slot + 1] - row0;
             for (int k = 0; k < m; ++k)
             {
-                constexpr int G = M8_I / 16 / 64;
-                const float* h = p.act + (size_t) (row0 + k) * p.I;
+                const unsigned long long* h = (const unsigned long long*) (p.act + (size_t) (row0 + k) * p.I);
                 float v[G][16];
                 uint32_t top = 0;
                 #pragma unroll
                 for (int g = 0; g < G; ++g)
-                    if (1024 * g < p.I) load16<HMOE_DT_F32, true>(h, min(l + 64 * g, p.I / 16 - 1), v[g]);
+                    if (1024 * g < p.I)
+                    {
+                        #pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                        {
+                            const unsigned long long u = __hip_atomic_load(h + 8 * min(l + 64 * g, p.I / 16 - 1) + j, __ATOMIC_RELAXED,
+                                                                           __HIP_MEMORY_SCOPE_AGENT);
+                            v[g][2 * j] = __uint_as_float((uint32_t) u);
+                            v[g][2 * j + 1] = __uint_as_float((uint32_t) (u >> 32));
+                        }
+                    }
                 #pragma unroll
                 for (int g = 0; g < G; ++g)
                     if (1024 * g < p.I)
@@ -537,11 +458,119 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
                             __hip_atomic_store(to + j, (unsigned long long) o[2 * j] | ((unsigned long long) o[2 * j + 1] << 32), __ATOMIC_RELAXED,
                                                __HIP_MEMORY_SCOPE_AGENT);
                     }
-                if (l == 0) __hip_atomic_store(p.sa + row0 + k, q.s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                if (l < M8_COPY)
+                    __hip_atomic_store(p.up + l * M8_ROWS + row0 + k, __float_as_uint(q.s) | 0x80000000u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (l == 0) __hip_atomic_store(p.flag + counted, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            counted = -1;
+        };
+        auto serve = [&]() __attribute__((always_inline)) {
+            if (head == tail) return;
+            const int slot = __builtin_amdgcn_readfirstlane((int) duty[head]);
+            const int v = l < M8_SUB ? __hip_atomic_load(p.count + 32 * (M8_SUB * slot + l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+            static_assert(M8_SUB == 8, "one 8-lane sum");
+            if (__builtin_amdgcn_readfirstlane(sum8(v)) != NB) return;
+            asm volatile("" ::: "memory");
+            quantise(slot);
+            ++head;
+        };
+        auto bring = [&](const Item& it) __attribute__((always_inline)) {
+            if (it.batch < 0 || it.ticket >= total || slots == 0) return;
+            const int s0 = it.batch * SB, s1 = min(s0 + SB, slots), r0 = s.row0[s0], n = s.row0[s1] - r0;
+            uint32_t v;
+            for (int polls = 0; !ask(it, v) && !lost; ++polls)
+            {
+                serve();
+                __builtin_amdgcn_s_sleep(2);
+                lost = polls > (1 << 22);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            int8_t* q = qb + (it.d & 1) * rq * QP;
+            const int pieces = n * (QP / 16);
+            for (int i0 = 0; i0 < pieces; i0 += 512)
+            {
+                u32x4 v[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                {
+                    const int i = min(i0 + 64 * j + l, pieces - 1);
+                    v[j] = ld16(p.qa + (size_t) (r0 + i / (QP / 16)) * IP + min(16 * (i % (QP / 16)), p.I - 16));
+                }
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                {
+                    const int i = i0 + 64 * j + l;
+                    if (i < pieces) *(u32x4*) (q + 16 * i) = 16 * (i % (QP / 16)) < p.I ? v[j] : (u32x4) {0u, 0u, 0u, 0u};
+                }
+            }
+            if (l < n) fq[it.d & 1][l] = lost ? __uint_as_float(0x7fc00000u) : __uint_as_float(v & 0x7fffffffu) * s.weight[r0 + l];
+        };
+        // the tickets to come: what is left of the run, then the claim that was made meanwhile
+        int left = first < 256 ? run - 1 : 0, last = start, nc = 0;
+        bool asked = false;
+        auto ticket = [&]() __attribute__((always_inline)) {
+            if (left > 0) { --left; last += 256; }
+            else
+            {
+                if (!asked && l == 0) nc = claim();
+                const int c = __builtin_amdgcn_readfirstlane(nc);
+                asked = false;
+                last = ticket_of(c);
+                left = c < 256 ? run - 1 : 0;
+            }
+            if (left <= 2 && last < NG && !asked)                        // (a down ticket takes long: no claim ahead of one)
+            {
+                if (l == 0) nc = claim();
+                asked = true;
+            }
+            return last;
+        };
+        if (cur.batch < 0 || nb == 1) tk[1] = ticket();
+        bring(cur);
+        __syncthreads();
+        while (cur.ticket < total)
+        {
+            // the ticket after the next; behind a down tile of several batches in its last but one
+            const Item nx = next(cur);
+            if (cur.batch < 0 && cur.ticket - cur.slot * NB == (int) ((uint32_t) (37 * cur.slot) % (uint32_t) NB)) duty[tail++] = (uint16_t) cur.slot;
+            serve();
+            if (cur.batch < 0 ? nx.batch < 0 || nb == 1 : nb == 1) tk[(cur.seq + 2) & 7] = ticket();
+            else if (cur.batch >= 0 && cur.batch == nb - 2) tk[(cur.seq + 1) & 7] = ticket();
+            const bool tn = turns(cur, nx);
+            uint32_t v;
+            const bool now = !tn || (apart && ask(nx, v));
+            if (now) bring(nx);
+            if (tn && l == 0) late = !now;
+            __syncthreads();
+            if (!now)
+            {
+                if (!apart) __syncthreads();
+                bring(nx);
+                __syncthreads();
+            }
+            cur = nx;
+        }
+        // what is left to quantise: its tiles are counted, or will be by workgroups that wait for nothing
+        for (int polls = 0; head < tail && polls < (1 << 22); ++polls) serve();
+        return;
+    }
+    if (w == 8)
+    {
+        // the finishing wave. A tile's values are stored in its item and counted in the next (behind the wait for that one's
+        // scales, which were asked for after them)
+        float sg = 0.f, su = 0.f;
+        auto scales = [&](const Item& it) {
+            if (it.batch >= 0 || it.ticket >= total || l >= 8 * TR) return;
+            const bool sh = p.hg && it.slot == 0;
+            const size_t so = (sh ? 0 : (size_t) s.expert[it.slot] * p.I) + min(8 * TR * it.blk + l, p.I - 1);
+            sg = (sh ? p.hsg : p.sg)[so];
+            su = (sh ? p.hsu : p.su)[so];
+        };
+        int stored = -1;                                                 // the ticket of the tile stored last
+        auto count = [&]() {
+            if (stored >= 0 && l == 0)
+                (void) __hip_atomic_fetch_add(p.count + 32 * (M8_SUB * (int) ((uint32_t) stored / (uint32_t) NB) + stored % M8_SUB), 1,
+                                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            stored = -1;
         };
         scales(cur);
         __syncthreads();
@@ -557,7 +586,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
                 // (values stored at the agent's scope go past the XCD's own L2: once the wait is over they can be seen, without
                 // writing the L2's lines back, which takes longer than a tile)
                 asm volatile("s_waitcnt vmcnt(0)" : "+v"(sg), "+v"(su) : : "memory");
-                look();
+                count();
                 for (int i0 = 0; i0 < 8 * TR * m; i0 += 64)
                 {
                     const int i = min(i0 + l, 8 * TR * m - 1), k = i / (8 * TR), rr = i - k * 8 * TR, n = 8 * TR * cur.blk + rr;
@@ -575,16 +604,13 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
                     if (i0 + l < 8 * TR * m && n < p.I)
                         __hip_atomic_store(p.act + (size_t) (row0 + k) * p.I + n, swiglu(g, u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                count();
-                stored = cur.slot;
+                stored = cur.ticket;
                 scales(nx);
                 if (nx.batch >= 0 || nx.ticket >= total)
                 {
                     // the last of this workgroup's gate/up tiles
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                    look();
                     count();
-                    look();
                 }
             }
             else if (cur.batch + 1 == nb)
@@ -612,12 +638,8 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         // (a pair behind the batch's last asks for one piece of x: every item has the same number of loads to wait for)
         DnAt o;
         o.live = 0;
-        int sl = 0, s1 = 0, og = 0;
-        if (slots > 0)
-        {
-            sl = __builtin_amdgcn_readfirstlane((int) bst[it.batch]);
-            s1 = __builtin_amdgcn_readfirstlane((int) bst[it.batch + 1]);
-        }
+        int sl = it.batch * SB, og = 0;
+        const int s1 = min(sl + SB, slots);
         #pragma unroll
         for (int b = 0; b < SU; ++b)
         {
@@ -626,8 +648,8 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
             if (sl < s1)
             {
                 const int e = expert_of(sl), n0 = 8 * min(RD * it.blk + og, p.H / 8 - 1);
-                wb = (e < 0 ? hd : wd + (size_t) e * p.H * p.I) + (size_t) n0 * p.I;
-                sb = (e < 0 ? hsd : wsd + (size_t) e * p.H) + n0;
+                wb = (const int8_t*) ((uintptr_t) p.wd + (e < 0 ? p.dd : (int64_t) e * p.H * p.I) + (size_t) n0 * p.I);
+                sb = (const float*) ((uintptr_t) p.sd + (e < 0 ? p.dsd : (int64_t) e * p.H * 4) + (size_t) n0 * 4);
                 o.live = b + 1;
             }
             o.w[b] = scalar(wb);
@@ -717,13 +739,8 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         float* acc = accl + ((it.seq & 1) * 8 + w) * 8 * RD * T;
         if (it.batch == 0)
             for (int i = l; i < 8 * RD * T; i += 64) acc[i] = 0.f;
-        int sl = 0, s1 = 0, r0 = 0, og = 0;
-        if (slots > 0)
-        {
-            sl = __builtin_amdgcn_readfirstlane((int) bst[it.batch]);
-            s1 = __builtin_amdgcn_readfirstlane((int) bst[it.batch + 1]);
-            r0 = s.row0[sl];
-        }
+        int sl = it.batch * SB, og = 0;
+        const int s1 = min(sl + SB, slots), r0 = s.row0[sl];
         const int8_t* qr = qb + (it.d & 1) * rq * QP + 128 * w * NSD + 16 * pc;
         const float* f = fq[it.d & 1];
         #pragma unroll
@@ -818,10 +835,9 @@ static void m8_launch(const M8Args& p, hipStream_t st)
 static size_t m8_layout(int T, int H, int I, int E, int topk, size_t* o)
 {
     const size_t rows = (size_t) T * (topk + 1);
-    const size_t part[] = {(size_t) T * E * 8, (size_t) T * up128(H), (size_t) T * 4, rows * I * 4, rows * up128(I), rows * 4,
-                           M8_SYNC * 4};
+    const size_t part[] = {(size_t) T * E * 8, (size_t) T * up128(H), (size_t) T * 4, rows * I * 4, rows * up128(I), M8_SYNC * 4};
     size_t at = 0;
-    for (int i = 0; i < 7; ++i)
+    for (int i = 0; i < 6; ++i)
     {
         if (o) o[i] = at;
         at += up128(part[i]);
@@ -868,15 +884,19 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
         const uintptr_t x0 = (uintptr_t) x, x1 = x0 + ((T - 1) * ldx + H) * ex, y0 = (uintptr_t) y, y1 = y0 + ((T - 1) * ldy + H) * ey;
         HMOE_REQUIRE(x1 <= y0 || y1 <= x0, "moe8_layer: the output overlaps x");
     }
-    size_t o[7];
+    size_t o[6];
     m8_layout(T, H, I, E, topk, o);
     uint8_t* b = (uint8_t*) work;
     M8Args p = {x, ldx, x_dtype, wr, bias, wg, wu, wd, sg, su, sd,
                 sh_w ? sh_w[0] : nullptr, sh_w ? sh_w[1] : nullptr, sh_w ? sh_w[2] : nullptr,
                 sh_s ? sh_s[0] : nullptr, sh_s ? sh_s[1] : nullptr, sh_s ? sh_s[2] : nullptr,
-                T, H, I, E, n, lo, topk, scale, sel, rw, y, ldy, y_dtype,
+                0, 0, 0, 0, T, H, I, E, n, lo, topk, scale, sel, rw, y, ldy, y_dtype,
                 (double*) (b + o[0]), (int8_t*) (b + o[1]), (float*) (b + o[2]), (float*) (b + o[3]), (int8_t*) (b + o[4]),
-                (float*) (b + o[5]), (int*) (b + o[6]), (int*) (b + o[6]) + 32, (int*) (b + o[6]) + 32 + 32 * M8_SLOTS};
+                (int*) (b + o[5]), (int*) (b + o[5]) + 32, (uint32_t*) (b + o[5]) + 32 + 32 * M8_SUB * M8_SLOTS};
+    p.dg = (int64_t) ((uintptr_t) p.hg - (uintptr_t) wg);
+    p.du = (int64_t) ((uintptr_t) p.hu - (uintptr_t) wu);
+    p.dd = (int64_t) ((uintptr_t) p.hd - (uintptr_t) wd);
+    p.dsd = (int64_t) ((uintptr_t) p.hsd - (uintptr_t) sd);
     const hipStream_t st = (hipStream_t) stream;
     const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * (x_dtype == HMOE_DT_F32 ? 4 : 2)) % 16 == 0;
 #define HMOE_R(D, V) m8_route_kernel<D, V><<<E + T, 256, 0, st>>>(p)
