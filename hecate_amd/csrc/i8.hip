@@ -1,6 +1,8 @@
 // i8.hip - products in 8-bit integers with a scale for each token and each output channel, and the gated MLP made of them
 // (hmoe_i8_quantize, hmoe_i8_matmul, hmoe_i8_linear, hmoe_i8_mlp):
 //   y[m][n] = s_x[m] s_w[n] sum_k q[m][k] w[n][k] (+ bias[n]), the sum exact in int32, the rest fp32, rounded once to y's type.
+// Few rows are brought into 8 bits by the product's own workgroups (i8_few.hip), others by a launch before it (i8_gemm1.hip,
+// i8_gemm2.hip: tiles out of LDS).
 #include "i8_gemm.h"
 
 namespace hmoe {
@@ -123,7 +125,9 @@ extern "C" int hmoe_i8_matmul(const int8_t* q, int64_t ldq, const float* s, int 
     HMOE_REQUIRE(((uintptr_t) bias & 3) == 0, "i8_matmul: bias alignment");
     if (int rc = check_y("i8_matmul", y, y_dtype, ldy, M, N)) return rc;
     HMOE_REQUIRE(!overlap(q, M, ldq, K, 1, y, M, ldy, N, dt_size(y_dtype)), "i8_matmul: the output overlaps q");
-    return i8_product(q, ldq, w, ldw, M, N, K, out_of(y, ldy, y_dtype, s, ws, nullptr, bias), (hipStream_t) stream);
+    const I8Out o = out_of(y, ldy, y_dtype, s, ws, nullptr, bias);
+    if (i8_few(M, N, K, 3)) return i8_few_product(q, 3, ldq, w, ldw, M, N, K, o, (hipStream_t) stream);
+    return i8_product(q, ldq, w, ldw, M, N, K, o, (hipStream_t) stream);
 }
 
 extern "C" size_t hmoe_i8_linear_work_bytes(int M, int N, int K)
@@ -146,8 +150,10 @@ extern "C" int hmoe_i8_linear(const void* x, int x_dtype, int64_t ldx, int M, co
     const hipStream_t st = (hipStream_t) stream;
     int8_t* q = (int8_t*) work;
     float* s = (float*) (q + up128((size_t) M * K));
+    const I8Out o = out_of(y, ldy, y_dtype, s, ws, nullptr, bias);
+    if (i8_few(M, N, K, x_dtype)) return i8_few_product(x, x_dtype, ldx, w, ldw, M, N, K, o, st);
     if (int rc = launch_quant(x, x_dtype, ldx, M, K, q, K, s, st)) return rc;
-    return i8_product(q, K, w, ldw, M, N, K, out_of(y, ldy, y_dtype, s, ws, nullptr, bias), st);
+    return i8_product(q, K, w, ldw, M, N, K, o, st);
 }
 
 // workspace: x in 8 bits and its scales, the gated rows in fp32, then in 8 bits with their scales
@@ -176,8 +182,17 @@ extern "C" int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H
     float* act = (float*) ((uint8_t*) s + up128((size_t) M * 4));
     int8_t* qa = (int8_t*) act + up128((size_t) M * Id * 4);
     float* sa = (float*) (qa + up128((size_t) M * Id));
-    if (int rc = launch_quant(x, x_dtype, ldx, M, Hd, q, Hd, s, st)) return rc;
-    if (int rc = i8_gated(q, Hd, wg, wu, Hd, M, Id, Hd, out_of(act, Id, HMOE_DT_F32, s, sg, su, nullptr), st)) return rc;
+    const I8Out up = out_of(act, Id, HMOE_DT_F32, s, sg, su, nullptr), down = out_of(y, ldy, y_dtype, sa, sd, nullptr, nullptr);
+    if (i8_few(M, Id, Hd, x_dtype))
+    {
+        if (int rc = i8_few_gated(x, x_dtype, ldx, wg, wu, Hd, M, Id, Hd, up, st)) return rc;
+    }
+    else
+    {
+        if (int rc = launch_quant(x, x_dtype, ldx, M, Hd, q, Hd, s, st)) return rc;
+        if (int rc = i8_gated(q, Hd, wg, wu, Hd, M, Id, Hd, up, st)) return rc;
+    }
+    if (i8_few(M, Hd, Id, HMOE_DT_F32)) return i8_few_product(act, HMOE_DT_F32, Id, wd, Id, M, Hd, Id, down, st);
     if (int rc = launch_quant(act, HMOE_DT_F32, Id, M, Id, qa, Id, sa, st)) return rc;
-    return i8_product(qa, Id, wd, Id, M, Hd, Id, out_of(y, ldy, y_dtype, sa, sd, nullptr, nullptr), st);
+    return i8_product(qa, Id, wd, Id, M, Hd, Id, down, st);
 }

@@ -27,6 +27,12 @@ int i8_product(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, int M
 int i8_gated(const int8_t* q, int64_t ldq, const int8_t* wg, const int8_t* wu, int64_t ldw, int M, int N, int K, const I8Out& o,
              hipStream_t st);
 
+// the same of few rows (i8_few.hip), of x as it is (src: its type; 3: in 8 bits, with the scales o.xs), where i8_few() holds
+bool i8_few(int M, int N, int K, int src);
+int i8_few_product(const void* x, int src, int64_t ldx, const int8_t* w, int64_t ldw, int M, int N, int K, const I8Out& o, hipStream_t st);
+int i8_few_gated(const void* x, int src, int64_t ldx, const int8_t* wg, const int8_t* wu, int64_t ldw, int M, int N, int K, const I8Out& o,
+                 hipStream_t st);
+
 // the tile shape of least estimated time: rounds of 256 workgroups, one a CU, each of the tile's f + s depth / 6144
 struct I8Pick
 {

@@ -276,3 +276,35 @@ def test_same_bits_every_time_captured_and_on_another_stream(dev):
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(outs[0], outs[2]) and torch.equal(lin[0], lin[2]), (M, k)
+
+
+# few rows (i8_few.hip): 8 and 16 weight rows a tile, one and several turns of the loads, several tiles a workgroup, tails of each
+FEW = [(1, 9, 40960), (1, 20, 16400), (2, 4101, 16000), (3, 100, 13312), (8, 9, 4112), (8, 6150, 1040), (7, 515, 5136), (9, 37, 5120), (12, 8200, 528),
+       (10, 77, 2576), (16, 30, 1536), (15, 8193, 1008), (16, 260, 2976), (5, 33, 9504)]
+
+
+@pytest.mark.parametrize("M,N,K", FEW)
+def test_few_rows(dev, M, N, K):
+    w, ws = weight(N, K, M + N)
+    for dtype, odt, pad in ((BF, F32, 0), (F16, BF, 8), (F32, F16, 1), (None, F32, 0)):
+        log("few", M, N, K, dtype, odt, pad)
+        bias = torch.randn(N, generator=torch.Generator().manual_seed(N)).to(dev) if pad else None
+        x = rows(M, K, dtype or BF, M + K, pad)
+        q, a = R.rows8(x)
+        buf = torch.full((M + 2, N + pad), 7.0, dtype=odt, device=dev)
+        if dtype is None:
+            q8, s = torch.zeros((M, K + 16), dtype=torch.int8, device=dev)[:, :K], torch.zeros(M, device=dev)
+            i8.quantize(x, q8, s)
+            i8.matmul(q8, s, w, ws, buf[1:M + 1, :N], bias)
+        else:
+            i8.linear(x, w, ws, buf[1:M + 1, :N], i8.linear_work(dev, M, N, K), bias)
+        torch.cuda.synchronize()
+        p = R.product(q, a, w, ws)
+        check_out(buf[1:M + 1, :N], p, p if bias is None else p + bias.double().cpu().numpy())
+        assert bool((buf[0] == 7.0).all()) and bool((buf[M + 1] == 7.0).all()) and bool((buf[:, N:] == 7.0).all())
+
+
+@pytest.mark.parametrize("M,H,I", [(1, 512, 9216), (3, 4096, 4112), (8, 1040, 2064), (12, 528, 4112), (16, 1024, 48), (9, 2064, 80)])
+def test_few_rows_of_the_mlp(dev, M, H, I):
+    test_mlp(dev, M, H, I, BF, F32)
+    test_mlp(dev, M, H, I, F32, F16)
