@@ -8,34 +8,54 @@
 namespace hmoe {
 
 // ---- rows to 8 bits ----------------------------------------------------------------------------------------------
-// One workgroup a row: the row's largest magnitude, then its values again (out of the caches) as whole numbers.
-template <int DT, bool VEC>
+// One workgroup a row: the row's largest magnitude, then its values as whole numbers. HOLD: the 16 values a thread of a row of
+// up to 4096 HOLD stay in registers between the two; a longer row (0) is read again, out of the caches.
+template <int DT, bool VEC, int HOLD>
 __global__ void __launch_bounds__(256) i8_quant_kernel(const void* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
                                                        int64_t ldq, float* __restrict__ s)
 {
     __shared__ uint32_t wmax[4];
-    const int t = threadIdx.x;
+    constexpr int G = HOLD > 0 ? HOLD : 1;
+    const int t = threadIdx.x, pieces = K / 16;
     const size_t row = blockIdx.x;
     const uint8_t* xr = (const uint8_t*) x + row * (size_t) ldx * (DT == HMOE_DT_F32 ? 4 : 2);
+    int8_t* qr = q + row * (size_t) ldq;
+    float v[G][16];
     uint32_t m = 0;
-    for (int i = t; i < K / 16; i += 256)
-    {
-        float v[16];
-        load16<DT, VEC>(xr, i, v);
+    auto largest = [&](const float (&u)[16]) __attribute__((always_inline)) {
         #pragma unroll
-        for (int j = 0; j < 16; ++j) m = max(m, mag(v[j]));
+        for (int j = 0; j < 16; ++j) m = max(m, mag(u[j]));
+    };
+    if constexpr (HOLD > 0)
+    {
+        #pragma unroll
+        for (int g = 0; g < G; ++g) load16<DT, VEC>(xr, min(t + 256 * g, pieces - 1), v[g]);      // (past the row: its last values)
+        #pragma unroll
+        for (int g = 0; g < G; ++g) largest(v[g]);
     }
+    else
+        for (int i = t; i < pieces; i += 256)
+        {
+            load16<DT, VEC>(xr, i, v[0]);
+            largest(v[0]);
+        }
     m = wave_ext_u32<true>(m);
     if ((t & 63) == 0) wmax[t >> 6] = m;
     __syncthreads();
     const RowQ p = row_q(max(max(wmax[0], wmax[1]), max(wmax[2], wmax[3])));
     if (t == 0) s[row] = p.s;
-    for (int i = t; i < K / 16; i += 256)
+    if constexpr (HOLD > 0)
     {
-        float v[16];
-        load16<DT, VEC>(xr, i, v);
-        *(u32x4*) (q + row * (size_t) ldq + 16 * (size_t) i) = quant16<DT>(v, p);
+        #pragma unroll
+        for (int g = 0; g < G; ++g)
+            if (t + 256 * g < pieces) *(u32x4*) (qr + 16 * (t + 256 * g)) = quant16<DT>(v[g], p);
     }
+    else
+        for (int i = t; i < pieces; i += 256)
+        {
+            load16<DT, VEC>(xr, i, v[0]);
+            *(u32x4*) (qr + 16 * (size_t) i) = quant16<DT>(v[0], p);
+        }
 }
 
 constexpr int I8_MAXK = 131056;              // 128 x 128 x K stays below 2^31
@@ -45,7 +65,13 @@ static int launch_quant(const void* x, int dt, int64_t ldx, int M, int K, int8_t
 {
     const size_t es = dt == HMOE_DT_F32 ? 4 : 2;
     const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * es) % 16 == 0;
-#define HMOE_Q(D, V) i8_quant_kernel<D, V><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s)
+#define HMOE_Q(D, V)                                                                                                   \
+    do                                                                                                                 \
+    {                                                                                                                  \
+        if (K <= 4096) i8_quant_kernel<D, V, 1><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                              \
+        else if (K <= 8192) i8_quant_kernel<D, V, 2><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                         \
+        else i8_quant_kernel<D, V, 0><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                                        \
+    } while (0)
     if (dt == HMOE_DT_F32) { if (vec) HMOE_Q(HMOE_DT_F32, true); else HMOE_Q(HMOE_DT_F32, false); }
     else if (dt == HMOE_DT_BF16) { if (vec) HMOE_Q(HMOE_DT_BF16, true); else HMOE_Q(HMOE_DT_BF16, false); }
     else { if (vec) HMOE_Q(HMOE_DT_F16, true); else HMOE_Q(HMOE_DT_F16, false); }
