@@ -274,7 +274,7 @@ __device__ __forceinline__ u32x4 ldw16_at(const void* base, uint32_t off)
 // work is a list of tickets, taken in order through one counter: first the gate/up tiles (8 TR gated values of one expert: slot
 // after slot, the shared expert first), then the down tiles (8 output columns, over every slot, a batch of slots at a time).
 //
-// Once a slot's gate/up tiles are counted, one workgroup quantises its rows and shows their scales; a down batch waits for its
+// Once a slot's gate/up tiles are counted, its rows are quantised, each by one workgroup, and their scales shown; a down batch waits for its
 // rows' scales. Those come from earlier claims alone, which are held by workgroups that run already; a workgroup waits for none
 // before all its gate/up tiles are counted, and quantises what is left to it while it waits. So every wait ends, whatever else is on the card and however many of this launch's workgroups have
 // started (all the same it is bounded: past the bound the output is NaN).
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     __shared__ M8Plan s;
     __shared__ __attribute__((aligned(16))) int8_t arena[M8_ARENA];
     __shared__ float fq[2][M8_RQ];
-    __shared__ uint16_t duty[M8_SLOTS];                                 // the slots this workgroup is to quantise
+    __shared__ uint16_t duty[M8_ROWS];                                  // the rows this workgroup is to quantise: M8_T slot + its number there
     __shared__ int tk[8], late;
     const int t = threadIdx.x, l = t & 63, r = l >> 3, pc = l & 7;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -414,63 +414,62 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
             v = l < n ? __hip_atomic_load(up + r0 + l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 1u;
             return __ballot(v == 0u) == 0ull;
         };
-        // The workgroup that took one certain tile of a slot, another one for each slot, brings the slot's rows into 8 bits once all
-        // its tiles are counted. (Left to whoever counts the last tile, the slowest workgroup gets every slot, and is slower for
-        // it.) The values come past this XCD's caches, as they were stored, and go the same way
+        // The workgroup that took one certain tile of a slot, another one for each of its rows, brings that row into 8 bits once all
+        // the slot's tiles are counted. (Left to whoever counts the last tile, the slowest workgroup gets every slot, and is slower
+        // for it.) The values come past this XCD's caches, as they were stored, and go the same way
         int head = 0, tail = 0;
-        auto quantise = [&](int slot) __attribute__((always_inline)) {
-            constexpr int G = M8_I / 16 / 64;
-            const int row0 = s.row0[slot], m = s.row0[slot + 1] - row0;
-            for (int k = 0; k < m; ++k)
-            {
-                const unsigned long long* h = (const unsigned long long*) (p.act + (size_t) (row0 + k) * p.I);
-                float v[G][16];
-                uint32_t top = 0;
-                #pragma unroll
-                for (int g = 0; g < G; ++g)
-                    if (1024 * g < p.I)
-                    {
-                        #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                        {
-                            const unsigned long long u = __hip_atomic_load(h + 8 * min(l + 64 * g, p.I / 16 - 1) + j, __ATOMIC_RELAXED,
-                                                                           __HIP_MEMORY_SCOPE_AGENT);
-                            v[g][2 * j] = __uint_as_float((uint32_t) u);
-                            v[g][2 * j + 1] = __uint_as_float((uint32_t) (u >> 32));
-                        }
-                    }
-                #pragma unroll
-                for (int g = 0; g < G; ++g)
-                    if (1024 * g < p.I)
-                    {
-                        #pragma unroll
-                        for (int j = 0; j < 16; ++j) top = max(top, mag(v[g][j]));
-                    }
-                const RowQ q = row_q(wave_ext_u32<true>(top));
-                #pragma unroll
-                for (int g = 0; g < G; ++g)
-                    if (1024 * g < p.I && l + 64 * g < p.I / 16)
-                    {
-                        const u32x4 o = quant16<HMOE_DT_BF16>(v[g], q);
-                        unsigned long long* to = (unsigned long long*) (p.qa + (size_t) (row0 + k) * IP + 16 * (l + 64 * g));
-                        #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            __hip_atomic_store(to + j, (unsigned long long) o[2 * j] | ((unsigned long long) o[2 * j + 1] << 32), __ATOMIC_RELAXED,
-                                               __HIP_MEMORY_SCOPE_AGENT);
-                    }
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                if (l < M8_COPY)
-                    __hip_atomic_store(p.up + l * M8_ROWS + row0 + k, __float_as_uint(q.s) | 0x80000000u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+        auto take = [&](const Item& it) __attribute__((always_inline)) {
+            const int m = __builtin_amdgcn_readfirstlane(s.row0[it.slot + 1] - s.row0[it.slot]);
+            const int at = it.ticket - it.slot * NB;
+            for (int j = 0; j < m; ++j)
+                if (at == (int) ((uint32_t) (37 * it.slot + 11 * j) % (uint32_t) NB)) duty[tail++] = (uint16_t) (it.slot * M8_T + j);
         };
         auto serve = [&]() __attribute__((always_inline)) {
             if (head == tail) return;
-            const int slot = __builtin_amdgcn_readfirstlane((int) duty[head]);
-            const int v = l < M8_SUB ? __hip_atomic_load(p.count + 32 * (M8_SUB * slot + l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+            const int d = __builtin_amdgcn_readfirstlane((int) duty[head]), slot = d / M8_T, row = __builtin_amdgcn_readfirstlane(s.row0[slot] + d % M8_T);
+            const int c = l < M8_SUB ? __hip_atomic_load(p.count + 32 * (M8_SUB * slot + l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
             static_assert(M8_SUB == 8, "one 8-lane sum");
-            if (__builtin_amdgcn_readfirstlane(sum8(v)) != NB) return;
+            if (__builtin_amdgcn_readfirstlane(sum8(c)) != NB) return;
             asm volatile("" ::: "memory");
-            quantise(slot);
+            constexpr int G = M8_I / 16 / 64;
+            const unsigned long long* h = (const unsigned long long*) (p.act + (size_t) row * p.I);
+            float v[G][16];
+            uint32_t top = 0;
+            #pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (1024 * g < p.I)
+                {
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                    {
+                        const unsigned long long u = __hip_atomic_load(h + 8 * min(l + 64 * g, p.I / 16 - 1) + j, __ATOMIC_RELAXED,
+                                                                       __HIP_MEMORY_SCOPE_AGENT);
+                        v[g][2 * j] = __uint_as_float((uint32_t) u);
+                        v[g][2 * j + 1] = __uint_as_float((uint32_t) (u >> 32));
+                    }
+                }
+            #pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (1024 * g < p.I)
+                {
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) top = max(top, mag(v[g][j]));
+                }
+            const RowQ q = row_q(wave_ext_u32<true>(top));
+            #pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (1024 * g < p.I && l + 64 * g < p.I / 16)
+                {
+                    const u32x4 o = quant16<HMOE_DT_BF16>(v[g], q);
+                    unsigned long long* to = (unsigned long long*) (p.qa + (size_t) row * IP + 16 * (l + 64 * g));
+                    #pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        __hip_atomic_store(to + j, (unsigned long long) o[2 * j] | ((unsigned long long) o[2 * j + 1] << 32), __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT);
+                }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (l < M8_COPY)
+                __hip_atomic_store(p.up + l * M8_ROWS + row, __float_as_uint(q.s) | 0x80000000u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             ++head;
         };
         auto bring = [&](const Item& it) __attribute__((always_inline)) {
@@ -488,18 +487,18 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
             const int pieces = n * (QP / 16);
             for (int i0 = 0; i0 < pieces; i0 += 512)
             {
-                u32x4 v[8];
+                u32x4 e[8];
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                 {
                     const int i = min(i0 + 64 * j + l, pieces - 1);
-                    v[j] = ld16(p.qa + (size_t) (r0 + i / (QP / 16)) * IP + min(16 * (i % (QP / 16)), p.I - 16));
+                    e[j] = ld16(p.qa + (size_t) (r0 + i / (QP / 16)) * IP + min(16 * (i % (QP / 16)), p.I - 16));
                 }
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                 {
                     const int i = i0 + 64 * j + l;
-                    if (i < pieces) *(u32x4*) (q + 16 * i) = 16 * (i % (QP / 16)) < p.I ? v[j] : (u32x4) {0u, 0u, 0u, 0u};
+                    if (i < pieces) *(u32x4*) (q + 16 * i) = 16 * (i % (QP / 16)) < p.I ? e[j] : (u32x4) {0u, 0u, 0u, 0u};
                 }
             }
             if (l < n) fq[it.d & 1][l] = lost ? __uint_as_float(0x7fc00000u) : __uint_as_float(v & 0x7fffffffu) * s.weight[r0 + l];
@@ -531,7 +530,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         {
             // the ticket after the next; behind a down tile of several batches in its last but one
             const Item nx = next(cur);
-            if (cur.batch < 0 && cur.ticket - cur.slot * NB == (int) ((uint32_t) (37 * cur.slot) % (uint32_t) NB)) duty[tail++] = (uint16_t) cur.slot;
+            if (cur.batch < 0) take(cur);
             serve();
             if (cur.batch < 0 ? nx.batch < 0 || nb == 1 : nb == 1) tk[(cur.seq + 2) & 7] = ticket();
             else if (cur.batch >= 0 && cur.batch == nb - 2) tk[(cur.seq + 1) & 7] = ticket();
