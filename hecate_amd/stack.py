@@ -10,7 +10,8 @@ fused (default), by row count:
             combine fused with the next layer's input norm (runtime/tier/cn.cu:48-103, hmoe_decode_combine_norm: the
             parts summed in order, h += them, xn of the next layer); after the last layer the plain output launch.
 Unfused: the residual + RMSNorm kernel, the router inside the decode layer, the output into y, and one final combine.
-All forms give the same bits. Static-shaped and allocation-free either way.
+All forms give the same bits. A stack with a layer whose shared expert is in 8 bits runs unfused: those rows are none of the
+launches' parts. Static-shaped and allocation-free either way.
 """
 import torch
 
@@ -42,6 +43,7 @@ class DecodeStack:
         self.h.copy_(self.x)
         st = stream_of(self.h.device)
         L = len(self.layers)
+        fused = fused and all(lay.shared8 is None for lay in self.layers)
         parts = fused and R > 1
         if parts:
             call("hmoe_residual_rmsnorm", ptr(self.h), None, ptr(self.norm_w[0]), R, float(self.eps), ptr(self.xn),

@@ -4,13 +4,14 @@ row-block planner of runtime/tier/rtx_split.py:236-255 (pick_groups), restated f
 
 Decode (<= 16 rows): router_fused (writes the f16 copy of x) -> moe4.forward (routed + shared expert into the
 fp32 accumulator) -> bf16 output (accumulator zeroed). Prefill: router -> device dispatch plan (no host sync) ->
-moe4p.forward (routed + shared) -> bf16 output. Every launch is static-shaped and allocation-free, so a whole step can
+moe4p.forward (routed + shared) -> bf16 output. A shared expert in 8 bits (shared_int8) runs as i8.mlp, its fp32 rows the
+ones that the routed experts are added to. Every launch is static-shaped and allocation-free, so a whole step can
 be captured in a hipGraph.
 """
 import numpy as np
 import torch
 
-from . import moe4, moe4p, moe4t, router
+from . import i8, moe4, moe4p, moe4t, router
 from ._lib import call, lib, on_device, ptr, stream_of
 
 H, I, TOPK = 6144, 2048, 8
@@ -213,6 +214,15 @@ def f16t_rows(t, N, K):
     return t.view(torch.float16).view(N // 16, K // 32, 4, 16, 8).permute(0, 3, 1, 2, 4).reshape(N, K).contiguous()
 
 
+def shared_int8(gate, up, down):
+    """a shared expert's matrices (gate, up [I, H], down [H, I], row-major bf16, fp16 or fp32 on the GPU) in 8 bits with a scale for
+    each row, as the reference keeps it (tier_split.py:252-263): the (wg, wu, wd, sg, su, sd) that MoELayer takes as its shared
+    expert"""
+    q = [i8.quantize(w, torch.empty(w.shape, dtype=torch.int8, device=w.device), torch.empty(w.shape[0], device=w.device))
+         for w in (gate, up, down)]
+    return tuple(w for w, _ in q) + tuple(s for _, s in q)
+
+
 class PrefillBuffers:
     """device buffers of a prefill chunk of up to T rows: selection, dispatch plan (hmoe_dispatch), GEMM scratch"""
 
@@ -235,14 +245,15 @@ class PrefillBuffers:
             self.shw = torch.empty(int(L.hmoe_shared_work_bytes(T)) // 4 + 64, dtype=torch.float32, device=dev)
         else:
             self.scr = moe4p.scratch(dev, F, T)
-        self._y = self._sh = None
+        self._y = self._sh = self._work8 = None
         self.out = z(T, H, dt=torch.bfloat16)
         self.xh = z(T, H, dt=torch.float16)                        # the router's f16 copy of x (the GEMM input)
         self.sel, self.rw = z(T, topk, dt=torch.int64), z(T, topk, dt=torch.float16)
         self.logits = z(int(L.hmoe_router_scratch_bytes(T, E)) // 4, dt=torch.float32)
 
     # The two fp32 [T, H] buffers are made on first use: a layer needs at most one of them (the long prefill with the ordered
-    # combine sh, if it has a shared expert; with the atomic one y; the short prefill neither), 201 MB at 8192 rows
+    # combine sh, if it has a shared expert; with the atomic one y; the short prefill neither, or sh for a shared expert in 8
+    # bits), 201 MB at 8192 rows
     @property
     def y(self):
         """fp32 accumulator [T, H], kept zeroed"""
@@ -255,10 +266,17 @@ class PrefillBuffers:
 
     @property
     def sh(self):
-        """the shared expert's rows [T, H] of the long prefill's ordered combine"""
+        """the shared expert's rows [T, H] of the long prefill's ordered combine, or of one in 8 bits"""
         if self._sh is None:
             self._sh = torch.empty((self.T, H), dtype=torch.float32, device=self.out.device)
         return self._sh
+
+    @property
+    def work8(self):
+        """the workspace of a shared expert in 8 bits"""
+        if self._work8 is None:
+            self._work8 = i8.mlp_work(self.out.device, self.T, H, I)
+        return self._work8
 
     def bounds(self, T):
         """(picks, row blocks) a chunk of T rows can reach at most: what its plan's consumers are given. Not the buffers' own
@@ -280,10 +298,12 @@ class PrefillBuffers:
 
 class MoELayer:
     """one routed int4 MoE layer: router (fp32 W_g [E, H], selection bias), resident experts for ids [lo, lo + n_hot)
-    (ExpertBank, local id = id - lo), optional F16T shared expert; max_rows bounds the prefill chunk"""
+    (ExpertBank, local id = id - lo), optional shared expert: three F16T matrices, or six tensors in 8 bits (shared_int8);
+    max_rows bounds the prefill chunk"""
 
     def __init__(self, wg, bias, bank, shared=None, lo=0, n_hot=None, topk=TOPK, scale=2.5, max_rows=16):
-        self.wg, self.bias, self.bank, self.shared = wg, bias, bank, shared
+        self.wg, self.bias, self.bank = wg, bias, bank
+        self.shared, self.shared8 = (None, tuple(shared)) if shared is not None and len(shared) == 6 else (shared, None)
         self.device = wg.device
         self.E = wg.shape[0]
         self.lo, self.n_hot = lo, bank.n if n_hot is None else n_hot
@@ -299,6 +319,9 @@ class MoELayer:
         self.out = torch.zeros((self.max_rows, H), dtype=torch.bfloat16, device=dev)
         self.scr = moe4.scratch(dev)
         self._pf = None
+        if self.shared8 is not None:
+            self.rows8 = torch.empty((16, H), dtype=torch.float32, device=dev)       # a step's shared rows
+            self.work8 = i8.mlp_work(dev, 16, H, I)
         self._shared_rows = None                                   # row-major copies of the shared expert (prefill)
 
     # ---- routing ---------------------------------------------------------------------------------------------
@@ -315,6 +338,8 @@ class MoELayer:
         gq, uq, dq, gs, us, ds = self.bank.tables()
         sh = self.shared if (with_shared and self.shared is not None) else (0, 0, 0)
         xh = self.xh if xh is None else xh
+        if with_shared and self.shared8 is not None:
+            y[:R].add_(self.mlp8(xh[:R], self.rows8[:R], self.work8))
         if events is None:
             moe4.forward(xh[:R], self.sel[:R], self.rw[:R], self.n_hot, gq, uq, dq, gs, us, ds, *self.scr, y, blocks,
                          0, self.lo, sh[0], sh[1], sh[2], 0, 0, 0)
@@ -327,11 +352,15 @@ class MoELayer:
         moe4.down(self.sel[:R], self.rw[:R], self.n_hot, dq, ds, act, y32, ctr_b, y, blocks, self.lo, sh[2])
         events[2].record()
 
+    def mlp8(self, x, rows, work):
+        """the shared expert in 8 bits of x's rows into fp32 rows"""
+        return i8.mlp(x, *self.shared8, rows, work)
+
     def decode(self, x, y=None, out=True, with_shared=True, phases=15, blocks=0):
         """the decode layer in four launches (hmoe_moe_decode_layer): router + routed + shared experts of x bf16
         [R, H]; returns the bf16 [R, H] output (out=True) and / or adds into the fp32 y. phases: bit mask of the
         launches (1 router, 2 shared + routed gate/up, 4 shared + routed down, 8 output) for callers that time them
-        apart"""
+        apart. A shared expert in 8 bits: all of it with 2, its rows the fp32 y of the launches, output and y from that"""
         R = x.shape[0]
         on_device("decode", x, self.wg, y)
         if not (1 <= R <= 16 and x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape[1] == H):
@@ -340,6 +369,18 @@ class MoELayer:
         sh = self.shared if (with_shared and self.shared is not None) else (None, None, None)
         act, gu32, ctr_a, y32, _ = self.scr
         o = self.out[:R] if out else None
+        if with_shared and self.shared8 is not None:
+            if y is None and not out:
+                raise RuntimeError("decode: neither y nor out")
+            rows = self.rows8[:R]
+            if phases & 2:
+                self.mlp8(x, rows, self.work8)
+            self.decode(x, rows, False, False, phases, blocks)
+            if phases & 8 and y is not None:
+                y[:R].add_(rows)
+            if phases & 8 and out:
+                moe4.finish_bf16(rows, R, o)
+            return o
         call("hmoe_moe_decode_layer", ptr(x), ptr(self.wg), ptr(self.bias), self.E, self.topk, float(self.scale),
              ptr(self.logits), ptr(self.sel), ptr(self.rw), R, self.n_hot, self.lo, ptr(gq), ptr(uq), ptr(dq), ptr(gs),
              ptr(us), ptr(ds), ptr(sh[0]), ptr(sh[1]), ptr(sh[2]), ptr(act), ptr(gu32), ptr(ctr_a), ptr(y32),
@@ -373,6 +414,11 @@ class MoELayer:
             # 1923 -> 1905 us, 4300 3606 -> 3575, 8192 6319 -> 6253
             fused = out_bf16 is not None and self.deterministic
             sh = None
+            if with_shared and self.shared8 is not None:
+                sh = self.mlp8(x, pf.sh[:T], pf.work8)
+                if not fused:
+                    y[:T].add_(sh)
+                    sh = None
             if fused and with_shared and self.shared is not None:
                 sh = pf.sh[:T]
                 moe4t.shared(x, *self.shared_rows(), pf.shw, sh, add=False)
@@ -383,6 +429,15 @@ class MoELayer:
             if not fused and with_shared and self.shared is not None:
                 moe4t.shared(x, *self.shared_rows(), pf.shw, y)
             return fused
+        if with_shared and self.shared8 is not None:
+            # the routed experts' fp32 form, added to the shared expert's rows
+            rows = self.mlp8(x, pf.sh[:T], pf.work8)
+            self.prefill_experts(x, rows, False)
+            if out_bf16 is None:
+                y[:T].add_(rows)
+            else:
+                moe4.finish_bf16(rows, T, out_bf16)
+            return out_bf16 is not None
         sh = self.shared_rows() if (with_shared and self.shared is not None) else None
         moe4p.forward(x, pf.tok, pf.eid, pf.wt, pf.rbt, gq, uq, dq, gs, us, ds, *pf.scr,
                       y if out_bf16 is None else None, inv=pf.inv[:T * self.topk], meta=pf.meta, topk=self.topk,
