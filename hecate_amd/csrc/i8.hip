@@ -10,7 +10,7 @@ namespace hmoe {
 // ---- rows to 8 bits ----------------------------------------------------------------------------------------------
 // One workgroup a row: the row's largest magnitude, then its values as whole numbers. HOLD: the 16 values a thread of a row of
 // up to 4096 HOLD stay in registers between the two; a longer row (0) is read again, out of the caches.
-template <int DT, bool VEC, int HOLD>
+template <int DT, int HOLD>
 __global__ void __launch_bounds__(256) i8_quant_kernel(const void* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
                                                        int64_t ldq, float* __restrict__ s)
 {
@@ -29,14 +29,14 @@ __global__ void __launch_bounds__(256) i8_quant_kernel(const void* __restrict__ 
     if constexpr (HOLD > 0)
     {
         #pragma unroll
-        for (int g = 0; g < G; ++g) load16<DT, VEC>(xr, min(t + 256 * g, pieces - 1), v[g]);      // (past the row: its last values)
+        for (int g = 0; g < G; ++g) load16<DT>(xr, min(t + 256 * g, pieces - 1), v[g]);      // (past the row: its last values)
         #pragma unroll
         for (int g = 0; g < G; ++g) largest(v[g]);
     }
     else
         for (int i = t; i < pieces; i += 256)
         {
-            load16<DT, VEC>(xr, i, v[0]);
+            load16<DT>(xr, i, v[0]);
             largest(v[0]);
         }
     m = wave_ext_u32<true>(m);
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256) i8_quant_kernel(const void* __restrict__ 
     else
         for (int i = t; i < pieces; i += 256)
         {
-            load16<DT, VEC>(xr, i, v[0]);
+            load16<DT>(xr, i, v[0]);
             *(u32x4*) (qr + 16 * (size_t) i) = quant16<DT>(v[0], p);
         }
 }
@@ -63,26 +63,23 @@ constexpr int64_t I8_MAXLD = 1 << 28;        // the product's kernel steps over 
 
 static int launch_quant(const void* x, int dt, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* s, hipStream_t st)
 {
-    const size_t es = dt == HMOE_DT_F32 ? 4 : 2;
-    const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * es) % 16 == 0;
-#define HMOE_Q(D, V)                                                                                                   \
+#define HMOE_Q(D)                                                                                                      \
     do                                                                                                                 \
     {                                                                                                                  \
-        if (K <= 4096) i8_quant_kernel<D, V, 1><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                              \
-        else if (K <= 8192) i8_quant_kernel<D, V, 2><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                         \
-        else i8_quant_kernel<D, V, 0><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                                        \
+        if (K <= 4096) i8_quant_kernel<D, 1><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                                 \
+        else if (K <= 8192) i8_quant_kernel<D, 2><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                            \
+        else i8_quant_kernel<D, 0><<<M, 256, 0, st>>>(x, ldx, K, q, ldq, s);                                           \
     } while (0)
-    if (dt == HMOE_DT_F32) { if (vec) HMOE_Q(HMOE_DT_F32, true); else HMOE_Q(HMOE_DT_F32, false); }
-    else if (dt == HMOE_DT_BF16) { if (vec) HMOE_Q(HMOE_DT_BF16, true); else HMOE_Q(HMOE_DT_BF16, false); }
-    else { if (vec) HMOE_Q(HMOE_DT_F16, true); else HMOE_Q(HMOE_DT_F16, false); }
+    if (dt == HMOE_DT_F32) HMOE_Q(HMOE_DT_F32);
+    else if (dt == HMOE_DT_BF16) HMOE_Q(HMOE_DT_BF16);
+    else HMOE_Q(HMOE_DT_F16);
 #undef HMOE_Q
     return HMOE_LAUNCHED("i8 quantize");
 }
 
 static I8Out out_of(void* y, int64_t ldy, int dt, const float* xs, const float* ws, const float* ws2, const float* bias)
 {
-    const bool vec = ((uintptr_t) y & 15) == 0 && (ldy * (dt == HMOE_DT_F32 ? 4 : 2)) % 16 == 0;
-    return {y, ldy, dt, xs, ws, ws2, bias, vec};
+    return {y, ldy, dt, xs, ws, ws2, bias};
 }
 
 static bool is_dt(int dt) { return dt == HMOE_DT_F32 || dt == HMOE_DT_BF16 || dt == HMOE_DT_F16; }

@@ -59,13 +59,7 @@ __device__ __forceinline__ uint32_t q8_wide(float x, const RowQ& p, double rd)
     return (uint32_t) (int) __builtin_rint(q1);
 }
 
-// ---- 8 or 16 values of a row as fp32 ----
-template <int DT> __device__ __forceinline__ float load1(const void* p, size_t i)
-{
-    if constexpr (DT == HMOE_DT_F32) return ldg<float>((const float*) p + i);
-    else if constexpr (DT == HMOE_DT_BF16) return bf2f(ldg<uint16_t>((const uint16_t*) p + i));
-    else return (float) __builtin_bit_cast(_Float16, ldg<uint16_t>((const uint16_t*) p + i));
-}
+// ---- values of a row as fp32 ----
 template <int DT> __device__ __forceinline__ void widen2(uint32_t v, float& lo, float& hi)
 {
     if constexpr (DT == HMOE_DT_BF16) { lo = __uint_as_float(v << 16); hi = __uint_as_float(v & 0xffff0000u); }
@@ -75,20 +69,21 @@ template <int DT> __device__ __forceinline__ void widen2(uint32_t v, float& lo, 
         lo = (float) h[0]; hi = (float) h[1];
     }
 }
-// 16 values at element 16 i of a row: VEC: by 16-byte loads (the row 16-byte aligned)
-template <int DT, bool VEC> __device__ __forceinline__ void load16(const void* row, int i, float (&v)[16])
+// 16-byte and 8-byte accesses at an element's own alignment (the hardware takes them at any; a row of an odd stride in 4-byte pieces
+// takes 3 times as long)
+typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// 16 (4) values at element 16 i (4 i) of a row
+template <int DT> __device__ __forceinline__ void load16(const void* row, int i, float (&v)[16])
 {
-    if constexpr (!VEC)
-    {
-        #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = load1<DT>(row, (size_t) 16 * i + j);
-    }
-    else if constexpr (DT == HMOE_DT_F32)
+    if constexpr (DT == HMOE_DT_F32)
     {
         #pragma unroll
         for (int j = 0; j < 4; ++j)
         {
-            const f32x4 u = ldg<f32x4>((const float*) row + (size_t) 16 * i + 4 * j);
+            const f32x4_4 u = *(const HMOE_GLOBAL f32x4_4*) ((const HMOE_GLOBAL float*) row + (size_t) 16 * i + 4 * j);
             #pragma unroll
             for (int k = 0; k < 4; ++k) v[4 * j + k] = u[k];
         }
@@ -98,10 +93,25 @@ template <int DT, bool VEC> __device__ __forceinline__ void load16(const void* r
         #pragma unroll
         for (int j = 0; j < 2; ++j)
         {
-            const u32x4 u = ld16((const uint16_t*) row + (size_t) 16 * i + 8 * j);
+            const u32x4_2 u = *(const HMOE_GLOBAL u32x4_2*) ((const HMOE_GLOBAL uint16_t*) row + (size_t) 16 * i + 8 * j);
             #pragma unroll
             for (int k = 0; k < 4; ++k) widen2<DT>(u[k], v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
         }
+    }
+}
+template <int DT> __device__ __forceinline__ void load4(const void* row, int i, float (&v)[4])
+{
+    if constexpr (DT == HMOE_DT_F32)
+    {
+        const f32x4_4 u = *(const HMOE_GLOBAL f32x4_4*) ((const HMOE_GLOBAL float*) row + (size_t) 4 * i);
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = u[k];
+    }
+    else
+    {
+        const u32x2_2 u = *(const HMOE_GLOBAL u32x2_2*) ((const HMOE_GLOBAL uint16_t*) row + (size_t) 4 * i);
+        widen2<DT>(u[0], v[0], v[1]);
+        widen2<DT>(u[1], v[2], v[3]);
     }
 }
 template <int DT> __device__ __forceinline__ u32x4 quant16(const float (&v)[16], const RowQ& p)

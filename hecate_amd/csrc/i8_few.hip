@@ -16,7 +16,7 @@ namespace hmoe {
 // upper left and lower right 8 x 8 are the sums of the one half of the depth and of the other (the rest is not used). 1 token, depth
 // 6144: 20000 channels 22.0 us (5.6 TB/s) and 28.1 in 16 rows, 6144 channels 9.5 and 12.3, 256 channels 4.3 and 6.0.
 constexpr int FEW_T = 16, FEW_LDS = 48 * 1024, FEW_NW = 8;
-template <int NMAT, int SRC, bool VEC, int HALF, int NL>
+template <int NMAT, int SRC, int HALF, int NL>
 __global__ void __launch_bounds__(64 * FEW_NW) __attribute__((amdgpu_waves_per_eu(4, 4)))
 i8_few_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ w, const int8_t* __restrict__ w2, int64_t ldw, int M, int N,
               int K, I8Out o)
@@ -73,7 +73,7 @@ i8_few_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict_
         for (int h = 0; h < HOLD; ++h)
         {
             const int i = min(t + 64 * FEW_NW * h, pieces - 1), r = i / per;
-            load16<SRC, VEC>((const uint8_t*) x + r * lb, i - r * per, v[h]);
+            load16<SRC>((const uint8_t*) x + r * lb, i - r * per, v[h]);
         }
         __builtin_amdgcn_sched_barrier(0);                              // (loads come back in order: x is not to wait for the weights)
         place(blockIdx.x);
@@ -104,7 +104,7 @@ i8_few_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict_
         {
             const int i = min(i0 + t, pieces - 1), r = i / per;
             float u[16];
-            load16<SRC, VEC>((const uint8_t*) x + r * lb, i - r * per, u);
+            load16<SRC>((const uint8_t*) x + r * lb, i - r * per, u);
             largest(u, r, i0 + t < pieces);
         }
         sync();
@@ -118,7 +118,7 @@ i8_few_kernel(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict_
         {
             const int r = i / per;
             float u[16];
-            load16<SRC, VEC>((const uint8_t*) x + r * lb, i - r * per, u);
+            load16<SRC>((const uint8_t*) x + r * lb, i - r * per, u);
             put(u, r, i - r * per);
         }
     }
@@ -201,24 +201,22 @@ template <int NMAT>
 static int launch_few(const void* x, int src, int64_t ldx, const int8_t* w, const int8_t* w2, int64_t ldw, int M, int N, int K, const I8Out& o,
                       hipStream_t st)
 {
-    const size_t es = src == 3 ? 1 : src == HMOE_DT_F32 ? 4 : 2;
-    const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * es) % 16 == 0;
     const FewPlan p = few_plan(NMAT, M, N, K);
-#define HMOE_N(S, V, H, L)                                                                                             \
+#define HMOE_N(S, H, L)                                                                                                \
     if (p.half == H && p.nl == L)                                                                                      \
-        i8_few_kernel<NMAT, S, V, H, L><<<p.grid, 64 * FEW_NW, p.lds, st>>>(x, ldx, w, w2, ldw, M, N, K, o);
-#define HMOE_F(S, V)                                                                                                   \
+        i8_few_kernel<NMAT, S, H, L><<<p.grid, 64 * FEW_NW, p.lds, st>>>(x, ldx, w, w2, ldw, M, N, K, o);
+#define HMOE_F(S)                                                                                                      \
     {                                                                                                                  \
-        HMOE_N(S, V, 0, 2) HMOE_N(S, V, 0, 4) HMOE_N(S, V, 0, 8) HMOE_N(S, V, 0, 12)                                   \
-        HMOE_N(S, V, 1, 1) HMOE_N(S, V, 1, 2) HMOE_N(S, V, 1, 4) HMOE_N(S, V, 1, 6)                                    \
+        HMOE_N(S, 0, 2) HMOE_N(S, 0, 4) HMOE_N(S, 0, 8) HMOE_N(S, 0, 12)                                               \
+        HMOE_N(S, 1, 1) HMOE_N(S, 1, 2) HMOE_N(S, 1, 4) HMOE_N(S, 1, 6)                                                \
     }
     if (src == 3)
     {
-        if constexpr (NMAT == 1) HMOE_F(3, true)
+        if constexpr (NMAT == 1) HMOE_F(3)
     }
-    else if (src == HMOE_DT_F32) { if (vec) HMOE_F(HMOE_DT_F32, true) else HMOE_F(HMOE_DT_F32, false) }
-    else if (src == HMOE_DT_BF16) { if (vec) HMOE_F(HMOE_DT_BF16, true) else HMOE_F(HMOE_DT_BF16, false) }
-    else { if (vec) HMOE_F(HMOE_DT_F16, true) else HMOE_F(HMOE_DT_F16, false) }
+    else if (src == HMOE_DT_F32) HMOE_F(HMOE_DT_F32)
+    else if (src == HMOE_DT_BF16) HMOE_F(HMOE_DT_BF16)
+    else HMOE_F(HMOE_DT_F16)
 #undef HMOE_F
 #undef HMOE_N
     return HMOE_LAUNCHED("i8 few rows");

@@ -19,7 +19,6 @@ struct I8Out
 {
     void* y; int64_t ldy; int dt;
     const float* xs; const float* ws; const float* ws2; const float* bias;
-    int vec;                        // 4 (bf16, f16: also 8) channels of a row may be stored at once: address and stride allow it
 };
 
 // y = the product of one matrix (i8_gemm1.hip), or silu(gate) up in fp32 (i8_gemm2.hip); ldq and ldw below 2^28
@@ -49,29 +48,33 @@ struct I8Pick
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// C (4 or 8) consecutive channels n .. of token m
+// C (4 or 8) consecutive channels n .. of token m, at once whatever the row's alignment
 template <int DT, int C, typename V>
 __device__ __forceinline__ void store_row(const I8Out& o, int m, int n, int N, const V& v)
 {
     const size_t at = (size_t) m * o.ldy + n;
-    if (o.vec && n + C <= N)
+    if (n + C <= N)
     {
         if constexpr (DT == HMOE_DT_F32)
         {
             #pragma unroll
-            for (int c = 0; c < C; c += 4) *(f32x4*) ((float*) o.y + at + c) = (f32x4) {v[c], v[c + 1], v[c + 2], v[c + 3]};
-        }
-        else if constexpr (C == 8)
-        {
-            if constexpr (DT == HMOE_DT_BF16) *(bf16x8*) ((uint16_t*) o.y + at) = __builtin_convertvector(v, bf16x8);
-            else *(f16x8*) ((uint16_t*) o.y + at) = __builtin_convertvector(v, f16x8);
+            for (int c = 0; c < C; c += 4)
+                *(HMOE_GLOBAL f32x4_4*) ((HMOE_GLOBAL float*) o.y + at + c) = (f32x4_4) {v[c], v[c + 1], v[c + 2], v[c + 3]};
         }
         else
         {
-            if constexpr (DT == HMOE_DT_BF16) *(bf16x4*) ((uint16_t*) o.y + at) = __builtin_convertvector(v, bf16x4);
-            else *(f16x4*) ((uint16_t*) o.y + at) = __builtin_convertvector(v, f16x4);
+            HMOE_GLOBAL uint16_t* to = (HMOE_GLOBAL uint16_t*) o.y + at;
+            if constexpr (C == 8)
+            {
+                if constexpr (DT == HMOE_DT_BF16) *(HMOE_GLOBAL u32x4_2*) to = __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
+                else *(HMOE_GLOBAL u32x4_2*) to = __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8));
+            }
+            else
+            {
+                if constexpr (DT == HMOE_DT_BF16) *(HMOE_GLOBAL u32x2_2*) to = __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
+                else *(HMOE_GLOBAL u32x2_2*) to = __builtin_bit_cast(u32x2, __builtin_convertvector(v, f16x4));
+            }
         }
         return;
     }

@@ -32,7 +32,7 @@ struct M8Args
 
 // ---- scores: one workgroup an expert, sums in 64 bits (scores next to each other decide the selection); behind them one
 // workgroup a token, that quantises its row ----
-template <int DT, bool VEC>
+template <int DT>
 __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
 {
     __shared__ double part[4][M8_T];
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
         for (int i = t; i < p.H / 16; i += 256)
         {
             float v[16];
-            load16<DT, VEC>(xr, i, v);
+            load16<DT>(xr, i, v);
             #pragma unroll
             for (int j = 0; j < 16; ++j) m = max(m, mag(v[j]));
         }
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
         for (int i = t; i < p.H / 16; i += 256)
         {
             float v[16];
-            load16<DT, VEC>(xr, i, v);
+            load16<DT>(xr, i, v);
             *(u32x4*) (p.xq + (size_t) row * up128(p.H) + 16 * i) = quant16<DT>(v, q);
         }
         return;
@@ -76,9 +76,10 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
         for (int r = 0; r < M8_T; ++r)
         {
             if (r >= p.T) break;
-            const uint8_t* xr = x + (size_t) r * p.ldx * es;
+            float v[4];
+            load4<DT>(x + (size_t) r * p.ldx * es, i, v);
             #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[r] = __builtin_fma((double) load1<DT>(xr, 4 * i + j), (double) wv[j], acc[r]);
+            for (int j = 0; j < 4; ++j) acc[r] = __builtin_fma((double) v[j], (double) wv[j], acc[r]);
         }
     }
     #pragma unroll
@@ -106,7 +107,8 @@ struct M8Plan
     float weight[M8_ROWS];
     float xs[M8_T];
     uint32_t scan[8];
-    int slots;
+    uint16_t batch[M8_SLOTS + 2];   // a down tile's batches: batch b holds the slots from batch[b] to batch[b + 1]
+    int slots, batches;
 };
 
 // a number ordered as the scores are, NaN behind everything
@@ -371,13 +373,13 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     m8_plan(p, s, blockIdx.x == 0);
     const int slots = __builtin_amdgcn_readfirstlane(s.slots);
     // a down tile: as many 8-row groups as give each of 256 workgroups one, so that the slots quantised last come last in it
-    const int RD = min(cdiv(p.H, 8 * 256), RDM), SB = max(min(SU / RD, rq / T), 1);
+    const int RD = min(cdiv(p.H, 8 * 256), RDM);
     const int NG = slots * NB, total = NG + cdiv(p.H, 8 * RD);
     // claims, one atomic each: the first 256 stand for `run` gate/up tiles, 256 apart (so that all work on the same slot), the
     // others for one ticket. (A claim for each tile from every workgroup kept one line of memory busy for longer than the tile)
     const int run = max(NG / 256 - 1, 1);
     auto ticket_of = [&](int c) { return c < 256 ? c : 256 * (run - 1) + c; };
-    const int nb = max(cdiv(slots, SB), 1);                             // batches of a down tile
+    int nb = 0;                                                         // batches of a down tile (from the first barrier below on)
 
     // an item: a gate/up tile (batch < 0) or one batch of a down tile; d counts the down items
     struct Item { int ticket, seq, slot, blk, batch, d; };
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         const uint32_t* up = p.up + (blockIdx.x % M8_COPY) * M8_ROWS;
         bool lost = false;
         auto ask = [&](const Item& it, uint32_t& v) __attribute__((always_inline)) {                    // whether the batch's rows are there; their scales
-            const int r0 = s.row0[it.batch * SB], n = s.row0[min((it.batch + 1) * SB, slots)] - r0;
+            const int r0 = s.row0[s.batch[it.batch]], n = s.row0[s.batch[it.batch + 1]] - r0;
             v = l < n ? __hip_atomic_load(up + r0 + l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 1u;
             return __ballot(v == 0u) == 0ull;
         };
@@ -474,7 +476,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         };
         auto bring = [&](const Item& it) __attribute__((always_inline)) {
             if (it.batch < 0 || it.ticket >= total || slots == 0) return;
-            const int s0 = it.batch * SB, s1 = min(s0 + SB, slots), r0 = s.row0[s0], n = s.row0[s1] - r0;
+            const int r0 = s.row0[s.batch[it.batch]], n = s.row0[s.batch[it.batch + 1]] - r0;
             uint32_t v;
             for (int polls = 0; !ask(it, v) && !lost; ++polls)
             {
@@ -523,6 +525,22 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
             }
             return last;
         };
+        // the batches of a down tile: up to SU / RD slots and rq rows (a slot has at most 16 of these). (With as many slots as would fit
+        // if every token were in each of them, 16 tokens over 102 experts of 6144 x 2048 took 708 us in place of 582, over 47 of
+        // 1840 x 288 146 in place of 84)
+        for (int at = 0; at < slots; ++nb)
+        {
+            const int c = min(at + 1 + l, slots);
+            const unsigned long long fit = __ballot(l < SU / RD && at + 1 + l <= slots && (int) s.row0[c] - (int) s.row0[at] <= rq);
+            if (l == 0) s.batch[nb] = (uint16_t) at;
+            at = __builtin_amdgcn_readfirstlane(at + max(__popcll(fit), 1));
+        }
+        if (l == 0)
+        {
+            s.batch[nb] = s.batch[nb + 1] = (uint16_t) slots;
+            s.batches = max(nb, 1);
+        }
+        nb = max(nb, 1);
         if (cur.batch < 0 || nb == 1) tk[1] = ticket();
         bring(cur);
         __syncthreads();
@@ -573,6 +591,7 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         };
         scales(cur);
         __syncthreads();
+        nb = __builtin_amdgcn_readfirstlane(s.batches);
         while (cur.ticket < total)
         {
             const Item nx = next(cur);
@@ -637,8 +656,8 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         // (a pair behind the batch's last asks for one piece of x: every item has the same number of loads to wait for)
         DnAt o;
         o.live = 0;
-        int sl = it.batch * SB, og = 0;
-        const int s1 = min(sl + SB, slots);
+        int sl = __builtin_amdgcn_readfirstlane((int) s.batch[it.batch]), og = 0;
+        const int s1 = __builtin_amdgcn_readfirstlane((int) s.batch[it.batch + 1]);
         #pragma unroll
         for (int b = 0; b < SU; ++b)
         {
@@ -738,8 +757,8 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         float* acc = accl + ((it.seq & 1) * 8 + w) * 8 * RD * T;
         if (it.batch == 0)
             for (int i = l; i < 8 * RD * T; i += 64) acc[i] = 0.f;
-        int sl = it.batch * SB, og = 0;
-        const int s1 = min(sl + SB, slots), r0 = s.row0[sl];
+        int sl = __builtin_amdgcn_readfirstlane((int) s.batch[it.batch]), og = 0;
+        const int s1 = __builtin_amdgcn_readfirstlane((int) s.batch[it.batch + 1]), r0 = s.row0[sl];
         const int8_t* qr = qb + (it.d & 1) * rq * QP + 128 * w * NSD + 16 * pc;
         const float* f = fq[it.d & 1];
         #pragma unroll
@@ -769,24 +788,22 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
     };
     GuAt ng;
     DnAt nd;
-    if (!early && cur.ticket < total)
+    if (!early && cur.batch < 0)
     {
-        if (cur.batch < 0)
-        {
-            ng = gu_at(expert_of(cur.slot), cur.blk);
+        ng = gu_at(expert_of(cur.slot), cur.blk);
+        #pragma unroll
+        for (int i = 0; i < NS; ++i)
             #pragma unroll
-            for (int i = 0; i < NS; ++i)
-                #pragma unroll
-                for (int tr = 0; tr < TR; ++tr) load_gu(ng, i, tr);
-        }
-        else
-        {
-            nd = dn_at(cur);
-            #pragma unroll
-            for (int j = 0; j < SU * NSD; ++j) load_dn(nd, j);
-        }
+            for (int tr = 0; tr < TR; ++tr) load_gu(ng, i, tr);
     }
     __syncthreads();
+    nb = __builtin_amdgcn_readfirstlane(s.batches);
+    if (cur.batch >= 0 && cur.ticket < total)
+    {
+        nd = dn_at(cur);
+        #pragma unroll
+        for (int j = 0; j < SU * NSD; ++j) load_dn(nd, j);
+    }
     Item nx = cur.ticket < total ? next(cur) : cur;
     if (cur.ticket < total && cur.batch < 0)
     {
@@ -897,12 +914,9 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
     p.dd = (int64_t) ((uintptr_t) p.hd - (uintptr_t) wd);
     p.dsd = (int64_t) ((uintptr_t) p.hsd - (uintptr_t) sd);
     const hipStream_t st = (hipStream_t) stream;
-    const bool vec = ((uintptr_t) x & 15) == 0 && (ldx * (x_dtype == HMOE_DT_F32 ? 4 : 2)) % 16 == 0;
-#define HMOE_R(D, V) m8_route_kernel<D, V><<<E + T, 256, 0, st>>>(p)
-    if (x_dtype == HMOE_DT_F32) { if (vec) HMOE_R(HMOE_DT_F32, true); else HMOE_R(HMOE_DT_F32, false); }
-    else if (x_dtype == HMOE_DT_BF16) { if (vec) HMOE_R(HMOE_DT_BF16, true); else HMOE_R(HMOE_DT_BF16, false); }
-    else { if (vec) HMOE_R(HMOE_DT_F16, true); else HMOE_R(HMOE_DT_F16, false); }
-#undef HMOE_R
+    if (x_dtype == HMOE_DT_F32) m8_route_kernel<HMOE_DT_F32><<<E + T, 256, 0, st>>>(p);
+    else if (x_dtype == HMOE_DT_BF16) m8_route_kernel<HMOE_DT_BF16><<<E + T, 256, 0, st>>>(p);
+    else m8_route_kernel<HMOE_DT_F16><<<E + T, 256, 0, st>>>(p);
     // the lines of a hidden row that a wave takes, and as many 8-row groups as make 8 to 14 loads of an item with them
     if (H <= 1024) m8_launch<1, 6>(p, st);
     else if (H <= 2048) m8_launch<2, 3>(p, st);
