@@ -422,9 +422,9 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
         int head = 0, tail = 0;
         auto take = [&](const Item& it) __attribute__((always_inline)) {
             const int m = __builtin_amdgcn_readfirstlane(s.row0[it.slot + 1] - s.row0[it.slot]);
-            const int at = it.ticket - it.slot * NB;
+            const int at = it.ticket - it.slot * NB, step = max(NB / M8_T, 1);
             for (int j = 0; j < m; ++j)
-                if (at == (int) ((uint32_t) (37 * it.slot + 11 * j) % (uint32_t) NB)) duty[tail++] = (uint16_t) (it.slot * M8_T + j);
+                if (at == (int) ((uint32_t) (37 * it.slot + step * j) % (uint32_t) NB)) duty[tail++] = (uint16_t) (it.slot * M8_T + j);
         };
         auto serve = [&]() __attribute__((always_inline)) {
             if (head == tail) return;
