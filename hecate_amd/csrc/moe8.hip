@@ -32,7 +32,7 @@ struct M8Args
 
 // ---- scores: one workgroup an expert, sums in 64 bits (scores next to each other decide the selection); behind them one
 // workgroup a token, that quantises its row ----
-template <int DT>
+template <int DT, int NI>
 __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
 {
     __shared__ double part[4][M8_T];
@@ -65,31 +65,51 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
         }
         return;
     }
+    // the expert's whole row is asked for at once (NI = H / 1024 rounded up loads a thread; a load at a time took 10.5 us of 256 x 6144
+    // and one token), then four tokens at a time
     const float* w = p.wr + (size_t) blockIdx.x * p.H;
-    double acc[M8_T];
+    const bool last = t + 256 * (NI - 1) < p.H / 4;                      // whether this thread has a part in the last load
+    f32x4 wv[NI];
     #pragma unroll
-    for (int r = 0; r < M8_T; ++r) acc[r] = 0.0;
-    for (int i = t; i < p.H / 4; i += 256)
-    {
-        const f32x4 wv = ldg<f32x4>(w + 4 * i);
+    for (int g = 0; g < NI; ++g) wv[g] = ldg<f32x4>(w + 4 * min(t + 256 * g, p.H / 4 - 1));
+    auto tokens = [&](auto many, int r0) __attribute__((always_inline)) {
+        constexpr int R = decltype(many)::value;
+        float v[R][NI][4];
         #pragma unroll
-        for (int r = 0; r < M8_T; ++r)
-        {
-            if (r >= p.T) break;
-            float v[4];
-            load4<DT>(x + (size_t) r * p.ldx * es, i, v);
+        for (int k = 0; k < R; ++k)
             #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[r] = __builtin_fma((double) v[j], (double) wv[j], acc[r]);
+            for (int g = 0; g < NI; ++g)
+                load4<DT>(x + (size_t) min(r0 + k, p.T - 1) * p.ldx * es, min(t + 256 * g, p.H / 4 - 1), v[k][g]);
+        double acc[R];
+        #pragma unroll
+        for (int k = 0; k < R; ++k)
+        {
+            acc[k] = 0.0;
+            #pragma unroll
+            for (int g = 0; g < NI; ++g)
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const double c = __builtin_fma((double) v[k][g][j], (double) wv[g][j], acc[k]);
+                    acc[k] = g < NI - 1 || last ? c : acc[k];
+                }
         }
-    }
-    #pragma unroll
-    for (int r = 0; r < M8_T; ++r)
-    {
-        if (r >= p.T) break;
-        double v = acc[r];
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-        if ((t & 63) == 0) part[t >> 6][r] = v;
-    }
+        for (int o = 32; o > 0; o >>= 1)
+        {
+            #pragma unroll
+            for (int k = 0; k < R; ++k) acc[k] += __shfl_xor(acc[k], o);
+        }
+        if ((t & 63) == 0)
+        {
+            #pragma unroll
+            for (int k = 0; k < R; ++k)
+                part[t >> 6][r0 + k] = acc[k];
+        }
+    };
+    if (p.T == 1) tokens(ic<1>{}, 0);
+    else
+        for (int r0 = 0; r0 < p.T; r0 += 4) tokens(ic<4>{}, r0);
+    static_assert(M8_T % 4 == 0, "part's room");
     __syncthreads();
     if (t < p.T) p.logits[(size_t) t * p.E + blockIdx.x] = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
 }
@@ -914,9 +934,14 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
     p.dd = (int64_t) ((uintptr_t) p.hd - (uintptr_t) wd);
     p.dsd = (int64_t) ((uintptr_t) p.hsd - (uintptr_t) sd);
     const hipStream_t st = (hipStream_t) stream;
-    if (x_dtype == HMOE_DT_F32) m8_route_kernel<HMOE_DT_F32><<<E + T, 256, 0, st>>>(p);
-    else if (x_dtype == HMOE_DT_BF16) m8_route_kernel<HMOE_DT_BF16><<<E + T, 256, 0, st>>>(p);
-    else m8_route_kernel<HMOE_DT_F16><<<E + T, 256, 0, st>>>(p);
+    const int ni = cdiv(H, 1024);
+#define HMOE_N(D, N) if (ni == N) m8_route_kernel<D, N><<<E + T, 256, 0, st>>>(p);
+#define HMOE_R(D) { HMOE_N(D, 1) HMOE_N(D, 2) HMOE_N(D, 3) HMOE_N(D, 4) HMOE_N(D, 5) HMOE_N(D, 6) HMOE_N(D, 7) }
+    if (x_dtype == HMOE_DT_F32) HMOE_R(HMOE_DT_F32)
+    else if (x_dtype == HMOE_DT_BF16) HMOE_R(HMOE_DT_BF16)
+    else HMOE_R(HMOE_DT_F16)
+#undef HMOE_R
+#undef HMOE_N
     // the lines of a hidden row that a wave takes, and as many 8-row groups as make 8 to 14 loads of an item with them
     if (H <= 1024) m8_launch<1, 6>(p, st);
     else if (H <= 2048) m8_launch<2, 3>(p, st);
