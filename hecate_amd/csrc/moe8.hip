@@ -39,10 +39,11 @@ __global__ void __launch_bounds__(256) m8_route_kernel(M8Args p)
     __shared__ uint32_t wmax[4];
     const int t = threadIdx.x, es = DT == HMOE_DT_F32 ? 4 : 2;
     const uint8_t* x = (const uint8_t*) p.x;
+    // (ticket, count, up: one array; by every workgroup: the tokens' own took 6 us for it at one token)
+    for (int i = blockIdx.x * 256 + t; i < M8_SYNC; i += gridDim.x * 256) p.ticket[i] = 0;
     if ((int) blockIdx.x >= p.E)
     {
         const int row = blockIdx.x - p.E;
-        for (int i = row * 256 + t; i < M8_SYNC; i += p.T * 256) p.ticket[i] = 0;      // (ticket, count, up: one array)
         const uint8_t* xr = x + (size_t) row * p.ldx * es;
         uint32_t m = 0;
         for (int i = t; i < p.H / 16; i += 256)
