@@ -9,7 +9,8 @@ namespace hmoe {
 
 // ---- rows to 8 bits ----------------------------------------------------------------------------------------------
 // One workgroup a row: the row's largest magnitude, then its values as whole numbers. HOLD: the 16 values a thread of a row of
-// up to 4096 HOLD stay in registers between the two; a longer row (0) is read again, out of the caches.
+// up to 4096 HOLD stay in registers between the two; a longer row (0) is read again, out of the caches. Bound by the bytes: 2048 rows
+// of 6144 in bf16 8 us (4.7 TB/s), fp32 rows of 2048 6 us; 61 rows 3.2 us, the launch and one round trip.
 template <int DT, int HOLD>
 __global__ void __launch_bounds__(256) i8_quant_kernel(const void* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
                                                        int64_t ldq, float* __restrict__ s)

@@ -8,6 +8,10 @@
 // of a fragment read lie on distinct banks. Each 64-k step's fragments are read one step ahead of its products. With WK > 1 the
 // waves' sums are joined in LDS.
 //
+// 8192 x 6144 of depth 2048 takes 120 us (1.72 POP/s), 2048 x 4096 of depth 6144 58 to 64 on different cards (1.6 to 1.8): the
+// matrix pipes are busy a third of that, the rest is fragment reads out of LDS and the stages' barriers. With few tiles the
+// stages' round trips bound it: 61 rows, 2048 channels, depth 6144 9.3 us, of which the bytes are 2.4.
+//
 // Where a wave has an even number of channel tiles, tiles 2 p and 2 p + 1 share 32 channels so that a lane's 4 rows of the one
 // and 4 of the other are 8 consecutive channels, stored at once.
 #pragma once

@@ -218,3 +218,16 @@ def test_rows_beside_the_output_stay(dev):
     out, sel, rw = L(x, F16, out=buf[1:4, :272])
     L.check(x, F16, (out, sel, rw))
     assert bool((buf[0] == 7).all()) and bool((buf[4] == 7).all()) and bool((buf[:, 272:] == 7).all())
+
+
+@pytest.mark.parametrize("E,n,lo,H,I,topk,shared", [(46, 46, 0, 1840, 288, 5, True), (16, 11, 3, 528, 496, 7, False), (12, 12, 0, 2576, 304, 3, True),
+                                                    (5, 5, 0, 4624, 112, 2, True), (200, 200, 0, 512, 1024, 8, True)])
+@pytest.mark.parametrize("T", [1, 4, 13, 16])
+def test_layer_of_many_rows(dev, E, n, lo, H, I, topk, shared, T):
+    """slots of one row and of many in the down batches, each number of loads of a router's row"""
+    log("layer of many rows", E, n, lo, H, I, topk, shared, T)
+    L = Layer(E, n, lo, H, I, topk, shared, E + H, dev)
+    x = rows(T, H, F16, T + H, dev, 5)
+    got = L(x, F32, L.work(T))
+    torch.cuda.synchronize()
+    L.check(x, F32, got)
