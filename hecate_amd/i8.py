@@ -19,6 +19,9 @@ from ._lib import check, lib, on_device
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the dtype codes of include/hecate_moe.h (HMOE_DT_*)
 
 
+_device, _stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _dt(what, t):
     d = _DT.get(t.dtype)
     if d is None:
@@ -28,12 +31,19 @@ def _dt(what, t):
 
 def _rows(what, t, M, K, dtype=None):
     """the row stride of a [M, K] tensor whose rows are contiguous"""
-    if t.shape != (M, K) or (K > 1 and t.stride(1) != 1) or (dtype is not None and t.dtype != dtype):
+    if t.shape != (M, K) or (dtype is not None and t.dtype != dtype):
         raise RuntimeError(f"{what} must be [{M}, {K}]{'' if dtype is None else ' ' + str(dtype)} with contiguous rows, "
                            f"got {tuple(t.shape)} {t.dtype}")
+    return _stride(what, t, M, K)
+
+
+def _stride(what, t, M, K):
+    """the same of a tensor whose shape is known"""
+    ld, step = t.stride()
+    if K > 1 and step != 1:
+        raise RuntimeError(f"{what} must be [{M}, {K}] with contiguous rows, got strides {t.stride()}")
     if M <= 1:
         return K
-    ld = t.stride(0)
     if ld < K:
         raise RuntimeError(f"{what}: rows overlap (stride {ld})")
     return ld
@@ -55,9 +65,25 @@ def _work(what, t, nbytes):
 
 
 def _two(what, x):
-    if x.dim() != 2:
-        raise RuntimeError(f"{what} must have two dimensions, got {tuple(x.shape)}")
-    return x.shape
+    sh = x.shape
+    if len(sh) != 2:
+        raise RuntimeError(f"{what} must have two dimensions, got {tuple(sh)}")
+    return sh
+
+
+def _on(what, x, *ts):
+    """on_device, by the devices' numbers where every argument is a tensor on the GPU"""
+    try:
+        i = x.get_device()
+        if i >= 0 and x.is_cuda:
+            for t in ts:
+                if t is not None and t.get_device() != i:
+                    break
+            else:
+                return
+    except AttributeError:
+        pass
+    on_device(what, x, *ts)
 
 
 @lru_cache(maxsize=256)
@@ -69,20 +95,20 @@ def _run(dev, name, *args):
     """the C entry on dev's current stream, with dev as the current device (raw queries: a call of a few microseconds pays
     for every Python object that it makes)"""
     i = dev.index
-    if i != torch._C._cuda_getDevice():
+    if i != _device():
         with torch.cuda.device(dev):
-            rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i))
+            rc = getattr(lib(), name)(*args, _stream(i))
     else:
-        rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i))
+        rc = getattr(lib(), name)(*args, _stream(i))
     if rc:
         check(rc, name)
 
 
 def quantize(x, q, s):
     """x [M, K] (bf16, fp16 or fp32) as int8 q [M, K] and fp32 scales s [M]"""
-    on_device("i8.quantize", x, q, s)
+    _on("i8.quantize", x, q, s)
     M, K = _two("i8: x", x)
-    ldx, ldq = _rows("i8.quantize: x", x, M, K), _rows("i8.quantize: q", q, M, K, torch.int8)
+    ldx, ldq = _stride("i8.quantize: x", x, M, K), _rows("i8.quantize: q", q, M, K, torch.int8)
     _vec("i8.quantize: s", s, M)
     _run(x.device, "hmoe_i8_quantize", x.data_ptr(), _dt("i8: x", x), ldx, M, K, q.data_ptr(), ldq, s.data_ptr())
     return q, s
@@ -90,10 +116,12 @@ def quantize(x, q, s):
 
 def matmul(q, s, w, ws, out, bias=None):
     """out [M, N] = s[m] ws[n] (q [M, K] w [N, K]^T) (+ bias [N] fp32) of rows that are in 8 bits already"""
-    on_device("i8.matmul", q, s, w, ws, out, bias)
+    _on("i8.matmul", q, s, w, ws, out, bias)
     M, K = _two("i8: q", q)
     N = _two("i8: w", w)[0]
-    ldq, ldy = _rows("i8.matmul: q", q, M, K, torch.int8), _rows("i8.matmul: out", out, M, N)
+    if q.dtype != torch.int8:
+        raise RuntimeError(f"i8.matmul: q must be int8, got {q.dtype}")
+    ldq, ldy = _stride("i8.matmul: q", q, M, K), _rows("i8.matmul: out", out, M, N)
     _mat("i8.matmul: w", w, N, K)
     _vec("i8.matmul: s", s, M)
     _vec("i8.matmul: ws", ws, N)
@@ -111,10 +139,10 @@ def linear_work(device, M, N, K):
 
 def linear(x, w, ws, out, work, bias=None):
     """out [M, N] = quantize(x [M, K]) w [N, K]^T (+ bias [N] fp32)"""
-    on_device("i8.linear", x, w, ws, out, work, bias)
+    _on("i8.linear", x, w, ws, out, work, bias)
     M, K = _two("i8: x", x)
     N = _two("i8: w", w)[0]
-    ldx, ldy = _rows("i8.linear: x", x, M, K), _rows("i8.linear: out", out, M, N)
+    ldx, ldy = _stride("i8.linear: x", x, M, K), _rows("i8.linear: out", out, M, N)
     _mat("i8.linear: w", w, N, K)
     _vec("i8.linear: ws", ws, N)
     if bias is not None:
@@ -133,10 +161,10 @@ def mlp_work(device, M, H, I):
 def mlp(x, wg, wu, wd, sg, su, sd, out, work):
     """out [M, H] = linear(h; wd, sd), h = silu(linear(x; wg, sg)) linear(x; wu, su) held in fp32 and quantised row by row;
     wg, wu int8 [I, H], wd int8 [H, I]"""
-    on_device("i8.mlp", x, wg, wu, wd, sg, su, sd, out, work)
+    _on("i8.mlp", x, wg, wu, wd, sg, su, sd, out, work)
     M, H = _two("i8: x", x)
     I = _two("i8.mlp: wg", wg)[0]
-    ldx, ldy = _rows("i8.mlp: x", x, M, H), _rows("i8.mlp: out", out, M, H)
+    ldx, ldy = _stride("i8.mlp: x", x, M, H), _rows("i8.mlp: out", out, M, H)
     _mat("i8.mlp: wg", wg, I, H)
     _mat("i8.mlp: wu", wu, I, H)
     _mat("i8.mlp: wd", wd, H, I)

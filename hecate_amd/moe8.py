@@ -17,8 +17,8 @@ import ctypes
 
 import torch
 
-from ._lib import on_device, ptr
-from .i8 import _bytes, _dt, _rows, _run, _two, _vec, _work
+from ._lib import ptr
+from .i8 import _bytes, _dt, _on, _rows, _run, _two, _vec, _work
 
 _P3 = ctypes.c_void_p * 3
 
@@ -38,7 +38,7 @@ def _w(what, t, shape, dtype):
 
 def layer(x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, scale, lo=0, shared=None):
     """one layer of x [T, H] (bf16, fp16 or fp32) into sel int64 [T, topk], rw fp32 [T, topk] and out [T, H]"""
-    on_device("moe8.layer", x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, *(shared or ()))
+    _on("moe8.layer", x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, *(shared or ()))
     T, H = _two("moe8.layer: x", x)
     E = _two("moe8.layer: wr", wr)[0]
     if wg.dim() != 3:
