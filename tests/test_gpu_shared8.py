@@ -136,3 +136,24 @@ def test_matrices_in_8_bits(layers):
         q, a = R8.rows8(m[:64])
         assert np.array_equal(lay.shared8[w8][:64].cpu().numpy().astype(np.float64), q)
         assert np.allclose(lay.shared8[s][:64].double().cpu().numpy(), a[:, 0] / 127.0, rtol=2.0 ** -24, atol=0)
+
+
+@pytest.mark.parametrize("T", [1, 6, 30])
+def test_captured(layers, T):
+    """decode (1, 6) and prefill (30) captured, replayed between eager calls of the same layer's twin"""
+    from hecate_amd import synth, tier
+    _, lay, _ = layers
+    twin = tier.MoELayer(lay.wg, lay.bias, lay.bank, lay.shared8, lo=0, n_hot=24)
+    x = synth.gen_x(3, T, lay.device)
+    lay.forward(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = lay.forward(x)
+    for k in range(3):
+        x.copy_(synth.gen_x(30 + k, T, lay.device))
+        want = twin.forward(x).clone()
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), k
