@@ -669,6 +669,9 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
                     float v = 0.f;
                     #pragma unroll
                     for (int k = 0; k < 8; ++k) v += ac[(k * 8 * RD + rr) * T + tok];
+                    // (a token that is not finite and has no expert here has no term that says so)
+                    const float xs = s.xs[tok];
+                    v = xs == xs ? v : xs;
                     if (8 * RD * cur.blk + rr < p.H) store_out(p.y, (size_t) tok * p.ldy + 8 * RD * cur.blk + rr, v, p.ydt);
                 }
             }
