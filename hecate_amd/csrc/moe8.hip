@@ -489,9 +489,10 @@ __global__ void __launch_bounds__(640) m8_experts_kernel(M8Args p)
             for (int g = 0; g < G; ++g)
                 if (1024 * g < p.I && l + 64 * g < p.I / 16)
                 {
-                    // (the quotient in 32 bits, not the 64 of an fp32 row that a caller gives: within 2^-23 of the true one, where the
-                    // gated value's own error is 2^-20 and more)
-                    const u32x4 o = quant16<HMOE_DT_BF16>(v[g], q);
+                    // (sixteen values at a time: all of a row's quotients in 64 bits at once spill the streaming waves' registers)
+                    __builtin_amdgcn_sched_barrier(0);
+                    const u32x4 o = quant16<HMOE_DT_F32>(v[g], q);
+                    __builtin_amdgcn_sched_barrier(0);
                     unsigned long long* to = (unsigned long long*) (p.qa + (size_t) row * IP + 16 * (l + 64 * g));
                     #pragma unroll
                     for (int j = 0; j < 2; ++j)

@@ -1,7 +1,11 @@
-"""The 8-bit expert layer (hecate_amd.moe8) on the GPU: rows that are not finite."""
+"""The 8-bit expert layer (hecate_amd.moe8) on the GPU: rows that are not finite, and the whole numbers of the gated rows."""
+from fractions import Fraction
+
+import numpy as np
 import pytest
 import torch
 
+from hecate_amd import i8, moe8
 from test_gpu_moe8 import BF, F16, F32, Layer, log, rows
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +30,34 @@ def test_rows_that_are_not_finite_without_a_resident_pick(dev, T, n):
         assert bool(o[bad].isnan().all())
         keep = [r for r in range(T) if r not in bad]
         assert torch.equal(o[keep], want.cpu()[keep].to(odt))
+
+
+def test_gated_rows_become_the_whole_numbers_of_the_mlp(dev):
+    """gated values next to the borders between whole numbers, in the layer and in the gated MLP: half to even of the true quotient.
+    x = (127, 64, 64, ..) has scale 1, so g = 64 / 2 = 32, silu(32) = 32 in fp32 (e^-32 < 2^-25), u = 64 su and h = 2048 su: any
+    fp32 value. With wd the identity an output is its gated row's whole number times the row's scale"""
+    H = I = 768
+    x = torch.full((1, H), 64.0, dtype=BF, device=dev)
+    x[0, 0] = 127.0
+    one = torch.zeros((I, H), dtype=torch.int8, device=dev)
+    one[:, 1] = 1
+    eye = torch.eye(H, I, dtype=torch.int8, device=dev)
+    sg, sd = torch.full((I,), 0.5, device=dev), torch.ones(H, device=dev)
+    for top in (3.4150088, 1.8574041, 1.1617918):
+        a = np.float32(top)
+        near = ((np.arange(127) + 0.5) * float(a) / 127).astype(np.float32)
+        h = np.concatenate([near, np.nextafter(near, np.float32(0)), np.nextafter(near, np.float32(9))])
+        h = np.concatenate([[a], h, -h, np.zeros(I - 1 - 2 * h.size, np.float32)]).astype(np.float32)
+        want = np.array([round(127 * Fraction(float(v)) / Fraction(float(a))) for v in h], dtype=np.float64)
+        su = torch.from_numpy(h / np.float32(2048)).to(dev)
+        y = torch.empty((1, H), device=dev)
+        i8.mlp(x, one, one, eye, sg, su, sd, y, i8.mlp_work(dev, 1, H, I))
+        s = float(a / np.float32(127))
+        assert np.array_equal(np.rint(y[0].double().cpu().numpy() / s), want)
+        # one expert, its weight 1: a / (a + 1e-20)
+        sel, rw, out = torch.empty((1, 1), dtype=torch.int64, device=dev), torch.empty((1, 1), device=dev), torch.empty((1, H), device=dev)
+        moe8.layer(x, torch.zeros((1, H), device=dev), None, one[None], one[None], eye[None], sg[None], su[None], sd[None], sel, rw, out,
+                   moe8.layer_work(dev, 1, H, I, 1, 1), 1.0)
+        assert float(rw) == 1.0
+        got = np.rint(out[0].double().cpu().numpy() / s)
+        assert np.array_equal(got, want), (int((got != want).sum()), "of", want.size)
