@@ -113,13 +113,6 @@ static int check_y(const char* what, const void* y, int dt, int64_t ldy, int M, 
     return HMOE_OK;
 }
 
-// whether rows a [n][cols] (row stride lda, es bytes an element) and b share a byte, by their whole spans
-static bool overlap(const void* a, int64_t n, int64_t lda, int64_t ca, int ea, const void* b, int64_t m, int64_t ldb, int64_t cb, int eb)
-{
-    const uintptr_t a0 = (uintptr_t) a, a1 = a0 + (size_t) ((n - 1) * lda + ca) * ea;
-    const uintptr_t b0 = (uintptr_t) b, b1 = b0 + (size_t) ((m - 1) * ldb + cb) * eb;
-    return a0 < b1 && b0 < a1;
-}
 static int dt_size(int dt) { return dt == HMOE_DT_F32 ? 4 : 2; }
 
 }  // namespace hmoe
@@ -133,7 +126,7 @@ extern "C" int hmoe_i8_quantize(const void* x, int x_dtype, int64_t ldx, int M, 
     if (int rc = check_x("i8_quantize", x, x_dtype, ldx, M, K)) return rc;
     HMOE_REQUIRE(q && s && ((uintptr_t) q & 15) == 0 && ((uintptr_t) s & 3) == 0 && ldq % 16 == 0 && rows_ok(M, ldq, K),
                  "i8_quantize: q: null, not 16-byte aligned, or row stride %lld", (long long) ldq);
-    HMOE_REQUIRE(!overlap(x, M, ldx, K, dt_size(x_dtype), q, M, ldq, K, 1), "i8_quantize: q overlaps x");
+    HMOE_REQUIRE(!rows_meet(M, x, ldx, K, dt_size(x_dtype), q, ldq, K, 1), "i8_quantize: q overlaps x");
     return launch_quant(x, x_dtype, ldx, M, K, q, ldq, s, (hipStream_t) stream);
 }
 
@@ -148,7 +141,7 @@ extern "C" int hmoe_i8_matmul(const int8_t* q, int64_t ldq, const float* s, int 
     if (int rc = check_w("i8_matmul", w, ws, ldw, N, K)) return rc;
     HMOE_REQUIRE(((uintptr_t) bias & 3) == 0, "i8_matmul: bias alignment");
     if (int rc = check_y("i8_matmul", y, y_dtype, ldy, M, N)) return rc;
-    HMOE_REQUIRE(!overlap(q, M, ldq, K, 1, y, M, ldy, N, dt_size(y_dtype)), "i8_matmul: the output overlaps q");
+    HMOE_REQUIRE(!rows_meet(M, q, ldq, K, 1, y, ldy, N, dt_size(y_dtype)), "i8_matmul: the output overlaps q");
     const I8Out o = out_of(y, ldy, y_dtype, s, ws, nullptr, bias);
     if (i8_few(M, N, K, 3)) return i8_few_product(q, 3, ldq, w, ldw, M, N, K, o, (hipStream_t) stream);
     return i8_product(q, ldq, w, ldw, M, N, K, o, (hipStream_t) stream);
@@ -169,7 +162,7 @@ extern "C" int hmoe_i8_linear(const void* x, int x_dtype, int64_t ldx, int M, co
     if (int rc = check_w("i8_linear", w, ws, ldw, N, K)) return rc;
     HMOE_REQUIRE(((uintptr_t) bias & 3) == 0, "i8_linear: bias alignment");
     if (int rc = check_y("i8_linear", y, y_dtype, ldy, M, N)) return rc;
-    HMOE_REQUIRE(!overlap(x, M, ldx, K, dt_size(x_dtype), y, M, ldy, N, dt_size(y_dtype)), "i8_linear: the output overlaps x");
+    HMOE_REQUIRE(!rows_meet(M, x, ldx, K, dt_size(x_dtype), y, ldy, N, dt_size(y_dtype)), "i8_linear: the output overlaps x");
     HMOE_REQUIRE(work && ((uintptr_t) work & 15) == 0, "i8_linear: workspace null or not 16-byte aligned");
     const hipStream_t st = (hipStream_t) stream;
     int8_t* q = (int8_t*) work;
@@ -198,7 +191,7 @@ extern "C" int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H
     if (int rc = check_w("i8_mlp", wu, su, Hd, Id, Hd)) return rc;
     if (int rc = check_w("i8_mlp", wd, sd, Id, Hd, Id)) return rc;
     if (int rc = check_y("i8_mlp", y, y_dtype, ldy, M, Hd)) return rc;
-    HMOE_REQUIRE(!overlap(x, M, ldx, Hd, dt_size(x_dtype), y, M, ldy, Hd, dt_size(y_dtype)), "i8_mlp: the output overlaps x");
+    HMOE_REQUIRE(!rows_meet(M, x, ldx, Hd, dt_size(x_dtype), y, ldy, Hd, dt_size(y_dtype)), "i8_mlp: the output overlaps x");
     HMOE_REQUIRE(work && ((uintptr_t) work & 15) == 0, "i8_mlp: workspace null or not 16-byte aligned");
     const hipStream_t st = (hipStream_t) stream;
     int8_t* q = (int8_t*) work;

@@ -165,6 +165,20 @@ __device__ __forceinline__ void store_out(void* out, size_t i, float v, int dt)
     else ((uint16_t*) out)[i] = to16(v, dt);
 }
 
+// whether M rows of ca values at a (row stride lda, ea bytes a value) and M rows at b share a byte: exactly where the rows lie the same
+// distance apart (column ranges of one buffer do), otherwise by their whole spans
+inline bool rows_meet(int64_t M, const void* a, int64_t lda, int64_t ca, int ea, const void* b, int64_t ldb, int64_t cb, int eb)
+{
+    const int64_t pa = lda * ea, pb = ldb * eb, wa = ca * ea, wb = cb * eb;
+    const uintptr_t a0 = (uintptr_t) a, b0 = (uintptr_t) b;
+    if (a0 + (uintptr_t) ((M - 1) * pa + wa) <= b0 || b0 + (uintptr_t) ((M - 1) * pb + wb) <= a0) return false;
+    if (M == 1 || pa != pb) return true;
+    // row j of b begins d + (j - i) pa bytes behind row i of a, and meets it if that is in (-wb, wa): the one distance in [0, pa), or
+    // the one before
+    const int64_t d = (int64_t) (b0 - a0), r = (d % pa + pa) % pa, k = (r - d) / pa;
+    return (r < wa && k > -M && k < M) || (r - pa > -wb && k - 1 > -M && k - 1 < M);
+}
+
 __host__ __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ __forceinline__ size_t up128(size_t n) { return (n + 127) & ~(size_t) 127; }
 

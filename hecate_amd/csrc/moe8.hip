@@ -928,11 +928,8 @@ extern "C" int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, c
     for (int i = 0; sh_w && i < 3; ++i)
         HMOE_REQUIRE(at(sh_w[i], 16) && at(sh_s[i], 4), "moe8_layer: shared expert: weights or scales null or not aligned");
     HMOE_REQUIRE(at(sel, 8) && at(rw, 4) && at(work, 128), "moe8_layer: sel, rw or workspace null or not aligned");
-    {
-        const int ex = x_dtype == HMOE_DT_F32 ? 4 : 2, ey = y_dtype == HMOE_DT_F32 ? 4 : 2;
-        const uintptr_t x0 = (uintptr_t) x, x1 = x0 + ((T - 1) * ldx + H) * ex, y0 = (uintptr_t) y, y1 = y0 + ((T - 1) * ldy + H) * ey;
-        HMOE_REQUIRE(x1 <= y0 || y1 <= x0, "moe8_layer: the output overlaps x");
-    }
+    HMOE_REQUIRE(!rows_meet(T, x, ldx, H, x_dtype == HMOE_DT_F32 ? 4 : 2, y, ldy, H, y_dtype == HMOE_DT_F32 ? 4 : 2),
+                 "moe8_layer: the output overlaps x");
     size_t o[6];
     m8_layout(T, H, I, E, topk, o);
     uint8_t* b = (uint8_t*) work;

@@ -256,7 +256,8 @@ int hmoe_shared_rows(const void* x, int T, const void* sh_gw, const void* sh_uw,
  * fp32 scale a row. y[m][n] = s[m] ws[n] sum_k q[m][k] w[n][k] (+ bias[n]): the sum exact in int32, the rest in fp32,
  * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131056; q, w and
  * the workspace are 16-byte aligned and their row strides multiples of 16 (below 2^28 in a product); x and y need their type's alignment only. M = 0 is
- * a no-op. y overlaps no input. ---- */
+ * a no-op. y overlaps no input: it may lie between x's rows as another column range of the same buffer; where the two row strides
+ * differ in bytes, outside x's whole span. ---- */
 /* x as q and s (the step that linear and mlp begin with, for a caller with several products of the same rows) */
 int hmoe_i8_quantize(const void* x, int x_dtype, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* s, void* stream);
 /* the product of rows that are in 8 bits already; bias fp32 [N] or NULL */
@@ -279,7 +280,7 @@ int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H, int I, co
  * their gated MLP (wg, wu [n][I][H], wd [n][H][I], scales [n][I], [n][I], [n][H]) and the shared expert's (sh_w / sh_s, host
  * arrays of three device addresses, gate, up, down; both NULL without one). T <= 16, topk <= 16, E <= 512, H and I multiples
  * of 16 up to 7168 and 4096. wr and the weights are 16-byte aligned, the workspace (hmoe_moe8_work_bytes, 0 for sizes that are refused)
- * 128-byte; a workspace made for more tokens serves fewer. T = 0 is a no-op. y overlaps no input. ---- */
+ * 128-byte; a workspace made for more tokens serves fewer. T = 0 is a no-op. y overlaps no input (as above). ---- */
 size_t hmoe_moe8_work_bytes(int T, int H, int I, int E, int topk);
 int hmoe_moe8_layer(const void* x, int x_dtype, int64_t ldx, int T, const float* wr, const float* bias, int E, int topk, double scale,
                     const int8_t* wg, const int8_t* wu, const int8_t* wd, const float* sg, const float* su, const float* sd, int n,
