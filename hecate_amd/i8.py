@@ -72,18 +72,19 @@ def _two(what, x):
 
 
 def _on(what, x, *ts):
-    """on_device, by the devices' numbers where every argument is a tensor on the GPU"""
+    """raise unless every argument is a tensor on x's GPU (on_device, by the devices' numbers); x stands for one that may be left out"""
     try:
         i = x.get_device()
         if i >= 0 and x.is_cuda:
             for t in ts:
-                if t is not None and t.get_device() != i:
+                if t.get_device() != i:
                     break
             else:
                 return
     except AttributeError:
         pass
     on_device(what, x, *ts)
+    raise RuntimeError(f"{what}: an argument that has to be a tensor is None or a number")
 
 
 @lru_cache(maxsize=256)
@@ -116,7 +117,7 @@ def quantize(x, q, s):
 
 def matmul(q, s, w, ws, out, bias=None):
     """out [M, N] = s[m] ws[n] (q [M, K] w [N, K]^T) (+ bias [N] fp32) of rows that are in 8 bits already"""
-    _on("i8.matmul", q, s, w, ws, out, bias)
+    _on("i8.matmul", q, s, w, ws, out, q if bias is None else bias)
     M, K = _two("i8: q", q)
     N = _two("i8: w", w)[0]
     if q.dtype != torch.int8:
@@ -139,7 +140,7 @@ def linear_work(device, M, N, K):
 
 def linear(x, w, ws, out, work, bias=None):
     """out [M, N] = quantize(x [M, K]) w [N, K]^T (+ bias [N] fp32)"""
-    _on("i8.linear", x, w, ws, out, work, bias)
+    _on("i8.linear", x, w, ws, out, work, x if bias is None else bias)
     M, K = _two("i8: x", x)
     N = _two("i8: w", w)[0]
     ldx, ldy = _stride("i8.linear: x", x, M, K), _rows("i8.linear: out", out, M, N)
