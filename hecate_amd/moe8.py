@@ -38,6 +38,8 @@ def _w(what, t, shape, dtype):
 
 def layer(x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, scale, lo=0, shared=None):
     """one layer of x [T, H] (bf16, fp16 or fp32) into sel int64 [T, topk], rw fp32 [T, topk] and out [T, H]"""
+    if shared is not None and len(shared) != 6:
+        raise RuntimeError(f"moe8.layer: shared must be six tensors (wg, wu, wd, sg, su, sd) or None, got {len(shared)}")
     _on("moe8.layer", x, wr, wg, wu, wd, sg, su, sd, sel, rw, out, x if bias is None else bias, x if work is None else work,
         *(shared or ()))
     T, H = _two("moe8.layer: x", x)

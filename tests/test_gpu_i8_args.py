@@ -39,3 +39,13 @@ def test_arguments_left_out(dev, name):
             with pytest.raises(RuntimeError, match="device"):
                 f(*args[:k], a.cpu(), *args[k + 1:])
     torch.cuda.synchronize()
+
+
+def test_shared_experts_of_another_number_of_tensors(dev):
+    f, args, _ = calls(dev)["layer"]
+    w = args[15]
+    for bad in ((), w[:3], w[:4], w[:5], w + (w[5],), w[0], w[:5] + (None,)):
+        with pytest.raises(RuntimeError):
+            f(*args[:15], bad)
+    f(*args[:15], list(w))
+    torch.cuda.synchronize()
