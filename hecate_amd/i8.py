@@ -16,6 +16,7 @@ import torch
 
 from ._lib import check, lib, on_device
 
+_MAX = (1 << 31) - 1                                                    # the C entries' sizes are 32-bit; a larger one would be cut to its low bits
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the dtype codes of include/hecate_moe.h (HMOE_DT_*)
 
 
@@ -68,6 +69,8 @@ def _two(what, x):
     sh = x.shape
     if len(sh) != 2:
         raise RuntimeError(f"{what} must have two dimensions, got {tuple(sh)}")
+    if sh[0] > _MAX or sh[1] > _MAX:
+        raise RuntimeError(f"{what}: {tuple(sh)}: more than {_MAX} rows or columns")
     return sh
 
 
@@ -89,6 +92,8 @@ def _on(what, x, *ts):
 
 @lru_cache(maxsize=256)
 def _bytes(name, *sizes):
+    if any(n > _MAX for n in sizes):
+        raise RuntimeError(f"{name}: a size of {sizes} is more than {_MAX}")
     return int(getattr(lib(), name)(*sizes))
 
 

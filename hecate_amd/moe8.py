@@ -48,6 +48,8 @@ def layer(x, wr, bias, wg, wu, wd, sg, su, sd, sel, rw, out, work, scale, lo=0, 
         raise RuntimeError(f"moe8.layer: wg must be [n, I, H], got {tuple(wg.shape)}")
     n, I = wg.shape[0], wg.shape[1]
     topk = _two("moe8.layer: sel", sel)[1]
+    if not 0 <= lo <= E - n:
+        raise RuntimeError(f"moe8.layer: resident experts [{lo}, {lo} + {n}) of {E}")
     ldx, ldy = _rows("moe8.layer: x", x, T, H), _rows("moe8.layer: out", out, T, H)
     i8, f32 = torch.int8, torch.float32
     for what, t, shape, dtype in (("wr", wr, (E, H), f32), ("wg", wg, (n, I, H), i8), ("wu", wu, (n, I, H), i8), ("wd", wd, (n, H, I), i8),

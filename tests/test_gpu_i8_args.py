@@ -49,3 +49,12 @@ def test_shared_experts_of_another_number_of_tensors(dev):
             f(*args[:15], bad)
     f(*args[:15], list(w))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lo", [1 << 32, -(1 << 32), (1 << 32) + 1, 1, -1])
+def test_first_resident_expert(dev, lo):
+    """lo is what it is, not its low 32 bits"""
+    f, args, _ = calls(dev)["layer"]
+    with pytest.raises(RuntimeError):
+        f(*args[:14], lo, args[15])
+    torch.cuda.synchronize()
