@@ -189,7 +189,8 @@ static FewPlan few_plan(int nmat, int M, int N, int K)
 // Where every workgroup's own quantisation costs less than a launch for it. Against that launch and the tiles of i8_gemm1.hip (us,
 // N = 6144, depth 2048): 1 row of bf16 5.9 and 9.1, 8 rows 6.7 and 9.5, 12 rows 9.0 and 9.6, 16 rows 10.8 and 9.7; of fp32 (in 64 bits:
 // twice the work) 8 rows 8.3 and 9.6, 12 rows 11.6 and 9.7; 16 rows that are in 8 bits already 6.3 and 7.1. Of depth 4096, 8 rows of
-// fp32 12.2 and 12.2; of depth 6144, 6 rows of bf16 12.7 and 14.6, 6 of fp32 15.1 and 14.8.
+// fp32 12.2 and 12.2; of depth 6144, 6 rows of bf16 12.7 and 14.6, 6 of fp32 15.1 and 14.8. The bounds do not look at N: both sides were
+// measured at 6144 channels only.
 bool i8_few(int M, int N, int K, int src)
 {
     if (M > FEW_T || few_plan(1, M, N, K).lds > FEW_LDS) return false;

@@ -5,12 +5,14 @@
 // in stages of 128 WK bytes: both operands' rows of a stage go to LDS by direct loads, whole 128-byte lines, in a ring of NST
 // stages issued NST - 1 ahead; one wait and barrier a stage. A stage holds each 8 rows' 128 bytes as a 1 KB block (block b: lane
 // l of its load takes row l / 8's 16-byte chunk (l % 8) ^ (l / 8) ^ 4 (b % 2), stored at 16 l), so that the 16 rows x 16 bytes
-// of a fragment read lie on distinct banks. Each 64-k step's fragments are read one step ahead of its products. With WK > 1 the
+// of a channel fragment's read lie on distinct banks where a wave has pairs of channel tiles. The other fragments' reads (the tokens',
+// and the channels' without pairs) take two lanes to each bank they touch: 4 cycles of conflict a read. Each 64-k step's fragments are read one step ahead of its products. With WK > 1 the
 // waves' sums are joined in LDS.
 //
-// 8192 x 6144 of depth 2048 takes 120 us (1.72 POP/s), 2048 x 4096 of depth 6144 58 to 64 on different cards (1.6 to 1.8): the
-// matrix pipes are busy a third of that, the rest is fragment reads out of LDS and the stages' barriers. With few tiles the
-// stages' round trips bound it: 61 rows, 2048 channels, depth 6144 9.3 us, of which the bytes are 2.4.
+// 8192 x 6144 of depth 2048 takes 122 us a call on operands that change from call to call (1.69 POP/s; 112 on the same ones again and
+// again, 134 as the profiler times the kernel), 2048 x 4096 of depth 6144 58 to 64 on different cards (1.6 to 1.8): the matrix pipes are
+// busy a third of that, the rest is fragment reads out of LDS and the stages' barriers. With few tiles the stages' round trips bound
+// it: 61 rows, 2048 channels, depth 6144 9.1 us, of which the bytes are 2.4.
 //
 // Where a wave has an even number of channel tiles, tiles 2 p and 2 p + 1 share 32 channels so that a lane's 4 rows of the one
 // and 4 of the other are 8 consecutive channels, stored at once.

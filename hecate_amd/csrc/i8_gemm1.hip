@@ -7,7 +7,10 @@ namespace hmoe {
 // depth / 6144 microseconds. Small tiles spread few rows over the chip and split the depth over the waves of a workgroup; large
 // ones read each operand less often. 16 x 16: 5.8 us at depth 6144 on 256 tiles (with 32 x 64 tiles the same product takes a
 // quarter of the workgroups and 11.8); 2048 x 4096 outputs of depth 6144: 57.8 us in 128 x 256 tiles, 70 in 192 x 256 (176 of
-// them), 78 in 128 x 128; 8192 x 6144 of depth 2048: 115 in 192 x 256, 130 in 128 x 256, 190 in 128 x 128.
+// them), 78 in 128 x 128; 8192 x 6144 of depth 2048: 115 in 192 x 256, 130 in 128 x 256, 190 in 128 x 128 (on the same operands again
+// and again). The constants rank the shapes; they are no launch's duration. A profiler shows 2 to 4 us more for the small ones: 9.1 us
+// for 61 x 2048 of depth 6144 (5.2 here), 9.5 for 333 x 1501 of depth 1360 (6.1), 9.7 for 77 x 6144 of depth 2048 (7.4); large ones
+// are within a tenth.
 #define HMOE_I8_SHAPES(X)                                                                                              \
     X(1, 1, 1, 1, 8, 3, 1.5f, 2.4f) X(2, 1, 1, 1, 8, 3, 2.2f, 3.0f) X(1, 2, 1, 1, 8, 3, 2.4f, 3.2f)                    \
     X(2, 2, 1, 1, 4, 4, 2.7f, 5.0f)                                                                                    \

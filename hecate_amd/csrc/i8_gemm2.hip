@@ -5,7 +5,7 @@
 namespace hmoe {
 
 // as in i8_gemm1.hip, channels counted in pairs: 2048 tokens, 2048 pairs of depth 6144 take 58 us in 64 x 256 tiles and 59 in
-// 128 x 128; 77 tokens 19 us in 16 x 48, 30 in 32 x 128
+// 128 x 128; 77 tokens 19 us in 16 x 48, 30 in 32 x 128 (by the constants 10.1; 14.3 as the profiler times the kernel alone)
 #define HMOE_I8_SHAPES(X)                                                                                              \
     X(2, 1, 1, 1, 8, 3, 2.2f, 3.2f) X(2, 2, 1, 1, 4, 4, 2.6f, 5.2f) X(2, 3, 1, 1, 4, 3, 3.5f, 6.6f)                    \
     X(2, 4, 1, 1, 4, 3, 4.1f, 7.6f) X(2, 4, 2, 1, 4, 2, 3.0f, 11.6f) X(2, 4, 2, 2, 2, 3, 4.4f, 16.8f)                  \

@@ -269,8 +269,9 @@ __device__ inline void m8_plan(const M8Args& p, M8Plan& s, bool write)
 }
 
 // the sum over the 8 lanes of a group, in each of them. v comes out of integer dot products, whose result another instruction
-// may read three wait states later at the earliest: where the two ended up in different blocks the compiler left two (the last
-// product was missing from the sum), so the wait is written out
+// may read three wait states later at the earliest. The compiler sees to that, copies that it makes itself included; the wait is
+// written out as well, from when a sum came out without its last product. (Followed along every path of the assembly of all the
+// kernels here, no result of a dot product is read earlier, with this wait or without it)
 __device__ __forceinline__ int sum8(int v)
 {
     asm volatile("s_nop 2" : "+v"(v));
@@ -313,7 +314,7 @@ __device__ __forceinline__ u32x4 ldw16_at(const void* base, uint32_t off)
 // waves load nothing else for the same reason, and the other two use what they ask for an item later.
 //
 // Measured with 256 experts of 6144 x 2048, top 8 and a shared one: 1 token 69 us of 340 MB (6.5 TB/s while it streams; 9 us go
-// before the first bytes, 5 between gate/up and down), 16 tokens 546 us of 3.9 GB (7.1 TB/s). With 5 tokens and experts of 2048 x
+// before the first bytes, 5 between gate/up and down), 16 tokens 536 us of the 3.3 GB of 86 distinct experts (6.1 TB/s). With 5 tokens and experts of 2048 x
 // 1408 (100 MB) the two gaps are half of 42 us.
 //
 // A wave's whole numbers are exact; those of a down tile are scaled and added slot by slot in fp32, then over the 8 waves: the

@@ -3,9 +3,9 @@
 Weights are int8 [N, K] row-major with one fp32 scale a row (the form in which the reference keeps its shared expert,
 runtime/tier/tier_split.py:252-263); rows of x are quantised on the fly: s = max |x| / 127, q = x / s rounded half to
 even. A row of zeros gives zeros; a row with a NaN or an infinity gives NaN in the whole output row. The integer sums are
-exact, everything else is fp32, and the output is rounded once to its type (bf16, fp16 or fp32). K is a multiple of 16;
-any number of rows, 0 included, and of output channels. x, q and out may have a row stride (x.stride(0)); w is
-contiguous.
+exact, everything else is fp32, and the output is rounded once to its type (bf16, fp16 or fp32). K is a multiple of 16 up to
+131056; rows up to 2^20, 0 included, output channels 1 to 2^20. x, q and out may have a row stride (x.stride(0); below 2^28 for
+the q of a product, and a multiple of 16 for any q), and be column ranges of one buffer; w is contiguous.
 
 Work runs on the current torch stream of x's device and allocates nothing; a workspace (linear_work, mlp_work) is the
 caller's, any contents work, and calls that share one must not overlap. Errors raise RuntimeError.

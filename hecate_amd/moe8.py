@@ -8,7 +8,8 @@
 
 Weights are int8 row-major: wg, wu [n, I, H], wd [n, H, I], fp32 scales sg, su [n, I], sd [n, H]; wr fp32 [E, H], bias fp32
 [E] or None; shared is None or (wg, wu, wd, sg, su, sd) of one expert without the leading axis. H and I are multiples of 16 up
-to 7168 and 4096, E at most 512, topk at most 16. A score that is NaN is selected last; a row with a NaN or an infinity gives NaN.
+to 7168 and 4096, E at most 512, topk at most 16. A score that is NaN is selected last; a row with a NaN or an infinity gives NaN,
+whether an expert of its own is resident or not.
 
 Work runs on the current torch stream of x's device and allocates nothing; the workspace (layer_work) is the caller's, any
 contents work, and calls that share one must not overlap. Errors raise RuntimeError.

@@ -252,8 +252,8 @@ class PrefillBuffers:
         self.logits = z(int(L.hmoe_router_scratch_bytes(T, E)) // 4, dt=torch.float32)
 
     # The two fp32 [T, H] buffers are made on first use: a layer needs at most one of them (the long prefill with the ordered
-    # combine sh, if it has a shared expert; with the atomic one y; the short prefill neither, or sh for a shared expert in 8
-    # bits), 201 MB at 8192 rows
+    # combine sh, if it has a shared expert; with the atomic one y; the short prefill neither), 201 MB at 8192 rows. A shared
+    # expert in 8 bits needs sh in every form, beside y in the atomic one
     @property
     def y(self):
         """fp32 accumulator [T, H], kept zeroed"""

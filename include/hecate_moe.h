@@ -254,8 +254,8 @@ int hmoe_shared_rows(const void* x, int T, const void* sh_gw, const void* sh_uw,
  * A row of x [M][K] is held as s = max |x| / 127 and q = 127 x / max |x| rounded half to even (a row of zeros: s = 0,
  * q = 0; a row with a NaN or an infinity: s = NaN, q = 0, so its products are NaN). Weights w int8 [N][K], row-major, one
  * fp32 scale a row. y[m][n] = s[m] ws[n] sum_k q[m][k] w[n][k] (+ bias[n]): the sum exact in int32, the rest in fp32,
- * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131056; q, w and
- * the workspace are 16-byte aligned and their row strides multiples of 16 (below 2^28 in a product); x and y need their type's alignment only. M = 0 is
+ * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131056, M at most and
+ * N 1 to 2^20; q, w and the workspace are 16-byte aligned and their row strides multiples of 16 (below 2^28 in a product); x and y need their type's alignment only. M = 0 is
  * a no-op. y overlaps no input: it may lie between x's rows as another column range of the same buffer; where the two row strides
  * differ in bytes, outside x's whole span. ---- */
 /* x as q and s (the step that linear and mlp begin with, for a caller with several products of the same rows) */
@@ -278,7 +278,8 @@ int hmoe_i8_mlp(const void* x, int x_dtype, int64_t ldx, int M, int H, int I, co
  * equal ones in the order of their ids, a NaN last; rw = scale a / (sum of the selected a + 1e-20), fp32 (the selection of
  * runtime/core/exl3_router.py:94-127). y [T][H] = the sum over the selected experts with lo <= id < lo + n of rw times
  * their gated MLP (wg, wu [n][I][H], wd [n][H][I], scales [n][I], [n][I], [n][H]) and the shared expert's (sh_w / sh_s, host
- * arrays of three device addresses, gate, up, down; both NULL without one). T <= 16, topk <= 16, E <= 512, H and I multiples
+ * arrays of three device addresses, gate, up, down; both NULL without one). A token that is not finite gives a row of NaN, with an
+ * expert here or without. T <= 16, topk <= 16, E <= 512, H and I multiples
  * of 16 up to 7168 and 4096. wr and the weights are 16-byte aligned, the workspace (hmoe_moe8_work_bytes, 0 for sizes that are refused)
  * 128-byte; a workspace made for more tokens serves fewer. T = 0 is a no-op. y overlaps no input (as above). ---- */
 size_t hmoe_moe8_work_bytes(int T, int H, int I, int E, int topk);
