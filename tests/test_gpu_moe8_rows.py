@@ -61,3 +61,11 @@ def test_gated_rows_become_the_whole_numbers_of_the_mlp(dev):
         assert float(rw) == 1.0
         got = np.rint(out[0].double().cpu().numpy() / s)
         assert np.array_equal(got, want), (int((got != want).sum()), "of", want.size)
+
+
+def test_no_tokens(dev):
+    """no tokens: nothing is launched, and no workspace is needed"""
+    L = Layer(8, 8, 0, 64, 32, 2, True, 23, dev)
+    out, sel, rw = L(torch.empty((0, 64), dtype=BF, device=dev), F32, work=L.work(4))
+    assert out.shape == (0, 64) and sel.shape == (0, 2) and rw.shape == (0, 2)
+    moe8.layer(out, L.wr.to(dev), None, *L.dw, *L.ds, sel, rw, torch.empty_like(out), None, 2.5)
