@@ -6,8 +6,8 @@
 // stages issued NST - 1 ahead; one wait and barrier a stage. A stage holds each 8 rows' 128 bytes as a 1 KB block (block b: lane
 // l of its load takes row l / 8's 16-byte chunk (l % 8) ^ (l / 8) ^ 4 (b % 2), stored at 16 l), so that the 16 rows x 16 bytes
 // of a channel fragment's read lie on distinct banks where a wave has pairs of channel tiles. The other fragments' reads (the tokens',
-// and the channels' without pairs) take two lanes to each bank they touch: 4 cycles of conflict a read. Each 64-k step's fragments are read one step ahead of its products. With WK > 1 the
-// waves' sums are joined in LDS.
+// and the channels' without pairs) take two lanes to each bank they touch: 4 cycles of conflict a read. Each 64-k step's fragments
+// are read one step ahead of its products. With WK > 1 the waves' sums are joined in LDS.
 //
 // 8192 x 6144 of depth 2048 takes 122 us a call on operands that change from call to call (1.69 POP/s; 112 on the same ones again and
 // again, 134 as the profiler times the kernel), 2048 x 4096 of depth 6144 58 to 64 on different cards (1.6 to 1.8): the matrix pipes are

@@ -314,8 +314,8 @@ __device__ __forceinline__ u32x4 ldw16_at(const void* base, uint32_t off)
 // waves load nothing else for the same reason, and the other two use what they ask for an item later.
 //
 // Measured with 256 experts of 6144 x 2048, top 8 and a shared one: 1 token 69 us of 340 MB (6.5 TB/s while it streams; 9 us go
-// before the first bytes, 5 between gate/up and down), 16 tokens 536 us of the 3.3 GB of 86 distinct experts (6.1 TB/s). With 5 tokens and experts of 2048 x
-// 1408 (100 MB) the two gaps are half of 42 us.
+// before the first bytes, 5 between gate/up and down), 16 tokens 536 us of the 3.3 GB of 86 distinct experts (6.1 TB/s).
+// With 5 tokens and experts of 2048 x 1408 (100 MB) the two gaps are half of 43 us.
 //
 // A wave's whole numbers are exact; those of a down tile are scaled and added slot by slot in fp32, then over the 8 waves: the
 // same order every time.

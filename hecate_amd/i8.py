@@ -16,7 +16,7 @@ import torch
 
 from ._lib import check, lib, on_device
 
-_MAX = (1 << 31) - 1                                                    # the C entries' sizes are 32-bit; a larger one would be cut to its low bits
+_MAX = (1 << 31) - 1                      # the C entries' sizes are 32-bit; a larger one would be cut to its low bits
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the dtype codes of include/hecate_moe.h (HMOE_DT_*)
 
 

@@ -255,9 +255,9 @@ int hmoe_shared_rows(const void* x, int T, const void* sh_gw, const void* sh_uw,
  * q = 0; a row with a NaN or an infinity: s = NaN, q = 0, so its products are NaN). Weights w int8 [N][K], row-major, one
  * fp32 scale a row. y[m][n] = s[m] ws[n] sum_k q[m][k] w[n][k] (+ bias[n]): the sum exact in int32, the rest in fp32,
  * rounded once to y's type. dtype codes HMOE_DT_*; row strides (ld*) in elements. K is a multiple of 16 up to 131056, M at most and
- * N 1 to 2^20; q, w and the workspace are 16-byte aligned and their row strides multiples of 16 (below 2^28 in a product); x and y need their type's alignment only. M = 0 is
- * a no-op. y overlaps no input: it may lie between x's rows as another column range of the same buffer; where the two row strides
- * differ in bytes, outside x's whole span. ---- */
+ * N 1 to 2^20; q, w and the workspace are 16-byte aligned and their row strides multiples of 16 (below 2^28 in a product); x and y
+ * need their type's alignment only. M = 0 is a no-op. y overlaps no input: it may lie between x's rows as another column range of
+ * the same buffer; where the two row strides differ in bytes, outside x's whole span. ---- */
 /* x as q and s (the step that linear and mlp begin with, for a caller with several products of the same rows) */
 int hmoe_i8_quantize(const void* x, int x_dtype, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* s, void* stream);
 /* the product of rows that are in 8 bits already; bias fp32 [N] or NULL */
